@@ -176,7 +176,8 @@ def run(state):
                                   label_smoothing=case["smoothing"], normalize_lengths=case["normalize"])
             return r.f, r.rewards, r.grad
         if case["op"] == "policy":
-            r = losses.policy(state["logps"], state["old"], state["advantages"], ref_logps=state["ref"], offsets=state["offsets"],
+            advantages = state["advantages"] if case["per_token"] else state["advantages"].unsqueeze(1)  # [sequences, 1]: one for each
+            r = losses.policy(state["logps"], state["old"], advantages, ref_logps=state["ref"], offsets=state["offsets"],
                               mask=state["mask"], clip_low=0.2, clip_high=0.28, kl_coef=case["kl"], reduction=case["reduction"])
             return r.f, r.kl, r.clip_fraction, r.grad
         return directions.orthogonalize(state["update"], steps=case["steps"], coefficients=NS)
