@@ -172,8 +172,9 @@ def run(state):
             logps, lse = losses.token_logprobs_with_lse(state["logits"], state["targets"], **kw)
             return logps, losses.token_logprobs_grad(state["logits"], state["targets"], lse, state["grad"], **kw)
         if case["op"] == "preference":
+            smoothing = case["smoothing"] if case["kind"] == "logistic" else 0.0  # the other kinds have none
             r = losses.preference(state["logps"], state["ref"], offsets=state["offsets"], mask=state["mask"], beta=0.1, kind=case["kind"],
-                                  label_smoothing=case["smoothing"], normalize_lengths=case["normalize"])
+                                  label_smoothing=smoothing, normalize_lengths=case["normalize"])
             return r.f, r.rewards, r.grad
         if case["op"] == "policy":
             advantages = state["advantages"] if case["per_token"] else state["advantages"].unsqueeze(1)  # [sequences, 1]: one for each
