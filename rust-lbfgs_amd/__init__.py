@@ -14,12 +14,12 @@ from .api import (BuiltinObjective, Context, DeviceEvaluate, TorchEvaluate, Lbfg
 
 
 def build(force=False):
-    """Compile liblbfgs_hip.so (hipcc, gfx950) and liblbfgs_solver.so (g++) in-tree."""
+    """Compile liblbfgs_hip.so and liblbfgs_train.so (hipcc, gfx950) and liblbfgs_solver.so (g++) in-tree."""
     return _build.build_all(force)
 
 
-def __getattr__(name):  # lazy submodules (dist imports torch)
-    if name in ("math", "objectives", "dist", "hotpath", "problem"):
+def __getattr__(name):  # lazy submodules (dist, losses and directions import torch)
+    if name in ("math", "objectives", "dist", "hotpath", "problem", "losses", "directions"):
         import importlib
 
         return importlib.import_module(f"{__name__}.{name}")

@@ -3,6 +3,7 @@
   liblbfgs_hip.so     HIP kernels + the C-ABI of include/lbfgs_hip.h   (hipcc, gfx950; three translation units:
                       csrc/context.hip, csrc/lbfgs_hip.hip, csrc/lj.hip, sharing csrc/ctx.h)
   liblbfgs_solver.so  host orchestration of include/lbfgs_solver.h    (g++, links the former)
+  liblbfgs_train.so   loss and update operators of include/lbfgs_train.h   (hipcc, gfx950; the units of csrc/train)
 
 hipcc cross-compiles for gfx950 without a GPU.  -ffp-contract=off on both sides: the
 reference's arithmetic is mul-then-add with separate roundings (src/math.rs:35,41).
@@ -23,6 +24,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 HIP_LIB = os.path.join(HERE, "liblbfgs_hip.so")
 SOLVER_LIB = os.path.join(HERE, "liblbfgs_solver.so")
+TRAIN_LIB = os.path.join(HERE, "liblbfgs_train.so")
+TRAIN_RESOURCES = os.path.join(HERE, "liblbfgs_train.resources.txt")
 RESOURCES = os.path.join(HERE, "liblbfgs_hip.resources.txt")  # per-kernel register / scratch usage of the last build
 
 # the library's translation units (compiled one by one, in parallel, then linked) ...
@@ -33,6 +36,10 @@ HIP_SRCS = HIP_UNITS + [os.path.join(CSRC, f) for f in ("ctx.h", "ops.h", "strea
 ]
 SOLVER_SRCS = [os.path.join(CSRC, "host", "solver.cpp"), os.path.join(ROOT, "include", "lbfgs_solver.h"),
                os.path.join(ROOT, "include", "lbfgs_hip.h")]
+
+TRAIN_UNITS = [os.path.join(CSRC, "train", f) for f in ("losses.hip", "logprobs.hip", "orthogonal.hip")]
+TRAIN_SRCS = TRAIN_UNITS + [os.path.join(CSRC, "train", "common.h"), os.path.join(ROOT, "include", "lbfgs_train.h"),
+                            os.path.join(ROOT, "include", "lbfgs_hip.h")]
 
 
 def source_hash(paths, flags=()):
@@ -62,12 +69,18 @@ def embedded_id(lib, marker):
 HIP_FLAGS = ["-O3", "--offload-arch=gfx950", "-ffp-contract=off", "-fPIC", "-std=c++17",
              # (resident.h parks data in the accumulation registers by hand: the compiler must not spill into them)
              "-mllvm", "-amdgpu-spill-vgpr-to-agpr=0", "-Wall"]
+# (32-bit arithmetic one value at a time: the packed forms the compiler makes by itself have given wrong results now and then)
+TRAIN_FLAGS = ["-O3", "--offload-arch=gfx950", "-fPIC", "-std=c++17", "-Wall", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 SOLVER_FLAGS = ["-O2", "-ffp-contract=off", "-fPIC", "-shared", "-std=c++17", "-Wall"]
 
 
 def hip_build_id():
     """What liblbfgs_hip.so must carry to belong to the checked-out sources."""
     return source_hash(HIP_SRCS, HIP_FLAGS)
+
+
+def train_build_id():
+    return source_hash(TRAIN_SRCS, TRAIN_FLAGS)
 
 
 def solver_build_id():
@@ -115,8 +128,8 @@ def _audit_agprs(asm_text):
 LAST_BUILD = {}  # name -> "compiled" | "reused" (what build_all did this time; __graft_entry__.build() prints it)
 
 
-def _compile_hip(out_lib, flags, build_id):
-    """Compile every unit of HIP_UNITS (in parallel: one hipcc -c each, in a directory of its own so that -save-temps keeps
+def _compile_hip(out_lib, flags, build_id, units=tuple(HIP_UNITS), marker="LBFGS_HIP_BUILD_ID"):
+    """Compile every unit of `units` (in parallel: one hipcc -c each, in a directory of its own so that -save-temps keeps
     the device assembly apart) and link them into `out_lib`.  -> (the compiler's per-kernel resource report, the AGPR audit).
     -Rpass-analysis=kernel-resource-usage: registers / scratch / occupancy of every kernel (tests/test_abi_exports.py requires
     ScratchSize == 0 everywhere: a kernel that touches scratch memory pays ~12 us of extra dispatch cost per launch on
@@ -129,15 +142,15 @@ def _compile_hip(out_lib, flags, build_id):
             os.makedirs(d)
             obj = os.path.join(d, "unit.o")
             r = _run([hipcc(), *flags, "-c", "-save-temps", "-Rpass-analysis=kernel-resource-usage",
-                      '-DLBFGS_HIP_BUILD_ID="%s"' % build_id, unit, "-o", obj], cwd=d)
+                      '-D%s="%s"' % (marker, build_id), unit, "-o", obj], cwd=d)
             asm = glob.glob(os.path.join(d, "*amdgcn*gfx950.s"))
             if len(asm) != 1:
                 raise RuntimeError("build: expected one device assembly file for %s, found %r" % (unit, asm))
             with open(asm[0]) as f:
                 return obj, r.stderr, f.read()
 
-        with ThreadPoolExecutor(max_workers=len(HIP_UNITS)) as ex:
-            results = list(ex.map(one, HIP_UNITS))
+        with ThreadPoolExecutor(max_workers=len(units)) as ex:
+            results = list(ex.map(one, units))
         _run([hipcc(), "--offload-arch=gfx950", "-fPIC", "-shared", *[o for o, _, _ in results], "-o", out_lib, "-ldl", "-lrt"])
         report = "".join(err for _, err, _ in results)
         audit = {}
@@ -177,7 +190,22 @@ def build_solver(force=False):
     return SOLVER_LIB
 
 
+def build_train(force=False):
+    want = train_build_id()
+    if force or _stale(TRAIN_LIB, "LBFGS_TRAIN_BUILD_ID", want) or not os.path.exists(TRAIN_RESOURCES):
+        report, _ = _compile_hip(TRAIN_LIB, TRAIN_FLAGS, want, TRAIN_UNITS, "LBFGS_TRAIN_BUILD_ID")
+        with open(TRAIN_RESOURCES, "w") as f:
+            f.write(report)
+        if embedded_id(TRAIN_LIB, "LBFGS_TRAIN_BUILD_ID") != want:
+            raise RuntimeError("build: %s does not carry the id it was built with" % TRAIN_LIB)
+        LAST_BUILD["liblbfgs_train.so"] = "compiled"
+    else:
+        LAST_BUILD.setdefault("liblbfgs_train.so", "reused")
+    return TRAIN_LIB
+
+
 def build_all(force=False):
+    build_train(force)
     return build_hip(force), build_solver(force)
 
 

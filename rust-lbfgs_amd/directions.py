@@ -1,0 +1,44 @@
+"""Directions for matrix parameters, beside the optimiser's own for vectors (the two-loop recursion, the orthant projection).
+
+    d = directions.orthogonalize(-gradient.view(rows, cols))      # every singular value brought near 1
+
+Kernels: rust-lbfgs_amd/csrc/train/orthogonal.hip behind include/lbfgs_train.h.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _train
+
+# a s + b s^3 + c s^5: the steepest start (3.44) whose iterates stay within 0.7 .. 1.2
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+def orthogonalize(update, *, steps=5, coefficients=COEFFICIENTS):
+    """`update` [..., rows, cols] (float32, bfloat16, float16) with its singular values brought near each other.
+
+    Each matrix is divided by its Frobenius norm (zeros stay zeros); then, `steps` times, every singular value s becomes
+    a s + b s^3 + c s^5 while the singular vectors stay: X <- (a I + b S + c S S) X with S = X X^T of the shorter side.  With the
+    default coefficients five steps bring all but the smallest (below a 1/1000 of the norm) into 0.7 .. 1.2.
+    Float32 and float16 results are those of 32-bit products, bfloat16 ones are within a rounding of them.
+    A matrix that holds a NaN or an infinity gives NaN, the others of its batch are not touched by it."""
+    _train.floating("update", update)
+    if update.dtype == torch.float64:
+        raise TypeError("update must be float32, bfloat16 or float16: the polynomial itself leaves singular values 20 % apart, "
+                        "64 bits have nothing to hold (convert it)")
+    if update.dim() < 2:
+        raise ValueError(f"update must be [..., rows, cols], not {tuple(update.shape)}")
+    if len(coefficients) != 3:
+        raise ValueError(f"coefficients are (a, b, c), not {coefficients!r}")
+    dev = _train.on_gpu(("update", update))
+    L = _train.load()
+    with _train.current(dev):
+        g = update.detach().contiguous()
+        out = torch.empty_like(g)
+        rows, cols = g.shape[-2:]
+        batch = g.numel() // (rows * cols) if rows and cols else 0
+        size = L.lbfgs_train_orthogonalize_workspace(batch, rows, cols)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+        _train.check(L.lbfgs_train_orthogonalize(_train.DTYPES[g.dtype], batch, rows, cols, g.data_ptr(), out.data_ptr(), steps, *coefficients,
+                                                 _train.ptr(ws), size, _train.stream_of(dev)))
+    return out

@@ -1,0 +1,228 @@
+"""Orthogonalised updates on the GPU against their definition in 64 bits.
+
+The tolerance follows the errors through the steps: what is rounded away before the last j steps, relative to |X|_F, is
+multiplied by at most the Lipschitz constant of the remaining map of the singular values (an odd function f acts on a matrix's
+singular values with the constant max |f'| in the Frobenius norm).  A step rounds S, P and X to 22 bits (2^-23 each, S and P
+acting through P's own size: counted 4 times) and accumulates in 32."""
+import math
+
+import pytest
+import torch
+
+from rust_lbfgs_amd import LbfgsError, directions
+
+pytestmark = pytest.mark.gpu
+DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+ABC = directions.COEFFICIENTS
+
+
+def in_64_bits(g, steps, abc):
+    x = g.double().cpu()
+    tall = x.shape[-2] > x.shape[-1]
+    x = x.mT if tall else x
+    n = x.square().sum((-2, -1), keepdim=True).sqrt()
+    x = torch.where(n > 0, x / n, 0.0)
+    a, b, c = abc
+    trail = [x]
+    for _ in range(steps):
+        s = x @ x.mT
+        x = a * x + (b * s + c * (s @ s)) @ x
+        trail.append(x)
+    return (x.mT if tall else x), trail
+
+
+def tolerance(g, trail, abc, dtype):
+    """Relative to the result, in the Frobenius norm, of the worst matrix of the batch."""
+    a, b, c = abc
+    worst = 0.0
+    flat = [t.reshape(-1, *t.shape[-2:]) for t in trail]
+    for k in range(flat[0].shape[0]):
+        norms = [float(t[k].norm()) for t in flat]
+        if not math.isfinite(norms[-1]) or norms[-1] == 0:
+            continue
+        off = 0.0
+        for j in range(len(flat)):
+            top = float(torch.linalg.matrix_norm(flat[j][k], 2)) if min(flat[j][k].shape) else 0.0
+            s = torch.linspace(0, top * 1.001 + 1e-12, 4001, dtype=torch.float64)
+            slope = torch.ones_like(s)
+            for _ in range(len(flat) - 1 - j):
+                slope = slope * (a + 3 * b * s ** 2 + 5 * c * s ** 4)
+                s = a * s + b * s ** 3 + c * s ** 5
+            scale = max(1.0, abs(a)) if j else 1.0
+            off += float(slope.abs().max()) * 12 * 2.0 ** -23 * scale * norms[j]
+            if dtype == torch.bfloat16 and j >= len(flat) - 3:  # 11-bit products near the end: 2^-12 each way, three products
+                off += float(slope.abs().max()) * 3 * 2.0 ** -12 * scale * norms[j]
+        worst = max(worst, off / norms[-1])
+    return worst + torch.finfo(dtype).eps / 2
+
+
+def check(g, steps=5, abc=ABC):
+    before = g.clone()
+    got = directions.orthogonalize(g, steps=steps, coefficients=abc)
+    assert torch.equal(g, before) and got.shape == g.shape and got.dtype == g.dtype and got.is_contiguous()
+    want, trail = in_64_bits(g, steps, abc)
+    tol = tolerance(g, trail, abc, g.dtype)
+    x, y = got.double().cpu().reshape(-1, *g.shape[-2:]), want.reshape(-1, *g.shape[-2:])
+    for k in range(x.shape[0]):
+        n = float(y[k].norm())
+        assert float((x[k] - y[k]).norm()) <= tol * n, (k, float((x[k] - y[k]).norm()) / n, tol)
+    return got, want
+
+
+def gradient(*shape, dtype=torch.float32, seed=0, rank=8, noise=0.3):
+    gen = torch.Generator().manual_seed(seed)
+    lead, (m, n) = shape[:-2], shape[-2:]
+    g = torch.randn(*lead, m, rank, generator=gen) @ torch.randn(*lead, rank, n, generator=gen) / math.sqrt(rank) + noise * torch.randn(*shape, generator=gen)
+    return g.to(dtype).cuda()
+
+
+SIZES = [(1, 1), (1, 9), (9, 1), (2, 3), (16, 16), (31, 33), (64, 64), (65, 63), (100, 300), (128, 128), (129, 127), (300, 128), (256, 512), (400, 401), (333, 1000)]
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("m, n", SIZES)
+def test_sizes(m, n, dtype):
+    check(gradient(m, n, dtype=DT[dtype]))
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("shape", [(3, 40, 50), (2, 3, 130, 70), (5, 200, 600), (1, 1, 20, 20), (17, 8, 8)])
+def test_batches(shape, dtype):
+    g = gradient(*shape, dtype=DT[dtype])
+    got, _ = check(g)
+    one = directions.orthogonalize(g.reshape(-1, *shape[-2:])[1 if g.numel() > shape[-1] * shape[-2] else 0])
+    assert torch.equal(one, got.reshape(-1, *shape[-2:])[1 if g.numel() > shape[-1] * shape[-2] else 0])  # a matrix is what it is alone
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("shape", [(700, 900), (1500, 500), (512, 2100), (1030, 1030)])
+def test_larger(shape, dtype):
+    check(gradient(*shape, dtype=DT[dtype], rank=32))
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("steps, abc", [(1, ABC), (2, ABC), (6, ABC), (8, (1.5, -0.5, 0.0)), (4, (15 / 8, -10 / 8, 3 / 8)), (3, (0.0, 0.0, 0.0)), (2, (-1.0, 0.0, 0.5)), (1, (1.0, 0.0, 0.0))])
+def test_steps_and_coefficients(steps, abc, dtype):
+    g = gradient(90, 140, dtype=DT[dtype])
+    got, want = check(g, steps, abc) if abc != (0.0, 0.0, 0.0) else (directions.orthogonalize(g, steps=steps, coefficients=abc), None)
+    if want is None:
+        assert (got == 0).all()
+
+
+@pytest.mark.parametrize("shape", [(60, 100), (200, 150), (256, 2000)])
+def test_low_rank_and_ill_conditioned(shape):
+    for dtype in DT.values():
+        check(gradient(*shape, dtype=dtype, rank=1, noise=0.0))
+        check(gradient(*shape, dtype=dtype, rank=4, noise=1e-3))
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_the_scale_of_an_update_does_not_matter(dtype):
+    t = DT[dtype]
+    g = gradient(70, 110, dtype=t)
+    want = directions.orthogonalize(g)
+    for k in (-12, 9) if t == torch.float16 else (-120, -60, 90):
+        h = g * 2.0 ** k
+        if torch.equal(h.double() * 2.0 ** -k, g.double()):
+            assert torch.equal(directions.orthogonalize(h), want), k
+        else:  # entries below the type's smallest normal number lost bits: another matrix
+            check(h)
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_zeros_and_bad_values_stay_with_their_matrix(dtype):
+    g = gradient(5, 60, 80, dtype=DT[dtype])
+    g[1] = 0
+    g[2, 3, 4] = math.nan
+    g[3, 0, 0] = math.inf
+    got = directions.orthogonalize(g)
+    assert (got[1] == 0).all() and got[2].isnan().all() and got[3].isnan().all()
+    for k in (0, 4):
+        assert torch.equal(got[k], directions.orthogonalize(g[k]))
+    assert directions.orthogonalize(torch.zeros(0, 3, 4, device="cuda")).shape == (0, 3, 4)
+    assert directions.orthogonalize(torch.zeros(3, 0, device="cuda")).shape == (3, 0)
+
+
+def test_strided_updates():
+    g = gradient(64, 200)
+    assert torch.equal(directions.orthogonalize(g[:, ::2]), directions.orthogonalize(g[:, ::2].contiguous()))
+    assert torch.equal(directions.orthogonalize(g.t()), directions.orthogonalize(g.t().contiguous()))
+    base = torch.zeros(64 * 100 + 1, device="cuda")
+    view = base[1:].view(64, 100)  # 4-byte aligned
+    view.copy_(g[:, :100])
+    assert torch.equal(directions.orthogonalize(view), directions.orthogonalize(g[:, :100].contiguous()))
+
+
+def test_a_tall_update_is_the_wide_ones_transpose():
+    for dtype in DT.values():
+        g = gradient(130, 300, dtype=dtype)
+        assert torch.equal(directions.orthogonalize(g.t().contiguous()), directions.orthogonalize(g).t())
+
+
+def test_other_streams_and_two_calls_at_once():
+    g, h = gradient(300, 500), gradient(4, 200, 200, dtype=torch.bfloat16)
+    want = directions.orthogonalize(g), directions.orthogonalize(h)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        got = []
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append((directions.orthogonalize(g), directions.orthogonalize(h)))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, want[0]) and torch.equal(b, want[1]) for a, b in got)
+
+
+def test_captured_and_replayed():
+    g, h = gradient(100, 150), gradient(3, 260, 200, dtype=torch.bfloat16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        directions.orthogonalize(g), directions.orthogonalize(h)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = directions.orthogonalize(g), directions.orthogonalize(h)
+        graphs.append((graph, out))
+    for k in range(4):
+        g.copy_(gradient(100, 150, seed=k + 3))
+        h.mul_(-1.5)
+        want = directions.orthogonalize(g), directions.orthogonalize(h)
+        for graph, out in graphs:
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+        torch.ones(1000, device="cuda").sum()
+
+
+def test_refusals_raise():
+    g = gradient(10, 10)
+    with pytest.raises(LbfgsError, match="steps"):
+        directions.orthogonalize(g, steps=0)
+    with pytest.raises(LbfgsError, match="out of range"):
+        directions.orthogonalize(g, coefficients=(5.0, 0.0, 0.0))
+    assert directions.orthogonalize(g).isfinite().all()
+
+
+def test_an_orthogonalised_descent_step():
+    """A step as it is used: gradient of a loss, momentum, the direction, the parameter."""
+    from rust_lbfgs_amd import losses
+
+    gen = torch.Generator().manual_seed(0)
+    W = torch.nn.Parameter((torch.randn(50, 24, generator=gen) * 0.1).cuda())
+    hidden, y = torch.randn(64, 24, generator=gen).cuda(), torch.randint(0, 50, (4, 16), generator=gen).cuda()
+    old = losses.token_logprobs((hidden @ W.detach().t()).view(4, 16, 50), y)
+    adv = torch.randn(4, 1, generator=gen).cuda()
+    momentum = torch.zeros_like(W)
+    for _ in range(3):
+        W.grad = None
+        losses.policy_loss(losses.token_logprobs((hidden @ W.t()).view(4, 16, 50), y), old, adv).backward()
+        momentum.mul_(0.9).add_(W.grad)
+        d = directions.orthogonalize(momentum)
+        want, trail = in_64_bits(momentum, 5, ABC)
+        assert float((d.double().cpu() - want).norm()) <= tolerance(momentum, trail, ABC, d.dtype) * float(want.norm())
+        with torch.no_grad():
+            W.sub_(0.02 * d)
+    assert W.isfinite().all()
