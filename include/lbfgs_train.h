@@ -106,9 +106,9 @@ int lbfgs_train_policy(const lbfgs_train_sequences* seqs, const void* logps, con
 /* ------------------------------------------------------------------------- */
 /* `batch` dense matrices rows x cols (F32, BF16, F16; batch <= 65535, sides <= 2^20): each is divided by its Frobenius norm (a
  * matrix of zeros stays one), and then `steps` times every singular value s becomes a s + b s^3 + c s^5, the singular vectors
- * staying as they are:  X <- (a I + b S + c S S) X, S = X X^T.  Products of 32-bit precision, except that the last steps of
- * BF16 updates use 16-bit ones.  Coefficients that lead a singular value of [0, 1] beyond 64 are refused. */
-uint64_t lbfgs_train_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols);
+ * staying as they are:  X <- (a I + b S + c S S) X, S = X X^T, in products of 32-bit precision.  Coefficients that lead a
+ * singular value of [0, 1] beyond 64, or multiply one by more than 16384 in all, are refused. */
+uint64_t lbfgs_train_orthogonalize_workspace(int32_t dtype, int64_t batch, int64_t rows, int64_t cols);
 int lbfgs_train_orthogonalize(int32_t dtype, int64_t batch, int64_t rows, int64_t cols, const void* update, void* out, int32_t steps,
                               double a, double b, double c, void* workspace, uint64_t workspace_bytes, void* stream);
 

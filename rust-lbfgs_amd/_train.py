@@ -41,7 +41,7 @@ SIGNATURES = {  # every symbol the header declares
     "lbfgs_train_sequences_workspace": (_u64, [_i64, _i64]),
     "lbfgs_train_preference": (C.c_int, [C.POINTER(Sequences), _vp, _vp, _d, _d, _i, _i, _vp, _vp, _vp, _vp, _u64, _vp]),
     "lbfgs_train_policy": (C.c_int, [C.POINTER(Sequences), _vp, _vp, _vp, _vp, _i, _d, _d, _d, _i, _vp, _vp, _vp, _vp, _vp, _u64, _vp]),
-    "lbfgs_train_orthogonalize_workspace": (_u64, [_i64, _i64, _i64]),
+    "lbfgs_train_orthogonalize_workspace": (_u64, [_i, _i64, _i64, _i64]),
     "lbfgs_train_orthogonalize": (C.c_int, [_i, _i64, _i64, _i64, _vp, _vp, _i, _d, _d, _d, _vp, _u64, _vp]),
 }
 

@@ -20,7 +20,7 @@ def orthogonalize(update, *, steps=5, coefficients=COEFFICIENTS):
     Each matrix is divided by its Frobenius norm (zeros stay zeros); then, `steps` times, every singular value s becomes
     a s + b s^3 + c s^5 while the singular vectors stay: X <- (a I + b S + c S S) X with S = X X^T of the shorter side.  With the
     default coefficients five steps bring all but the smallest (below a 1/1000 of the norm) into 0.7 .. 1.2.
-    Float32 and float16 results are those of 32-bit products, bfloat16 ones are within a rounding of them.
+    Products have 32-bit precision for all types; the result is rounded once.
     A matrix that holds a NaN or an infinity gives NaN, the others of its batch are not touched by it."""
     _train.floating("update", update)
     if update.dtype == torch.float64:
@@ -37,7 +37,7 @@ def orthogonalize(update, *, steps=5, coefficients=COEFFICIENTS):
         out = torch.empty_like(g)
         rows, cols = g.shape[-2:]
         batch = g.numel() // (rows * cols) if rows and cols else 0
-        size = L.lbfgs_train_orthogonalize_workspace(batch, rows, cols)
+        size = L.lbfgs_train_orthogonalize_workspace(_train.DTYPES[g.dtype], batch, rows, cols)
         ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         _train.check(L.lbfgs_train_orthogonalize(_train.DTYPES[g.dtype], batch, rows, cols, g.data_ptr(), out.data_ptr(), steps, *coefficients,
                                                  _train.ptr(ws), size, _train.stream_of(dev)))

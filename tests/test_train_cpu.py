@@ -161,8 +161,8 @@ def test_c_orthogonalize_refusals(lib):
     refused(call(abc=(-8.0, 0.0, 4000.0)), "out of range")
     refused(call(g=None), "are needed")
     refused(call(ws=None), "workspace")
-    refused(call(size=lib.lbfgs_train_orthogonalize_workspace(1, 4, 4) - 1), "workspace")
-    assert lib.lbfgs_train_orthogonalize_workspace(0, 4, 4) == 0
+    refused(call(size=lib.lbfgs_train_orthogonalize_workspace(1, 1, 4, 4) - 1), "workspace")
+    assert lib.lbfgs_train_orthogonalize_workspace(1, 0, 4, 4) == lib.lbfgs_train_orthogonalize_workspace(0, 1, 4, 4) == 0
     assert call(batch=0, g=None, out=None, ws=None) == 0 and call(m=0, g=None, out=None, ws=None) == 0
 
 
