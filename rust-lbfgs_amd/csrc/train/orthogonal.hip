@@ -164,54 +164,63 @@ __device__ __forceinline__ int place(int row, int chunk) {
     return chunk ^ (BK == 32 ? (row >> 1) & 3 : row & 7);
 }
 
-// One such copy: 16 bytes a lane from base + off to 1024 adjacent bytes of LDS.  Written out, because the compiler takes any LDS
-// read behind its own form of it as one that has to wait for all copies; the waits are the kernel's (ready()).
-__device__ __forceinline__ void copy_to_lds(const f16* from, uint32_t off, uint32_t lds) {
-    const uint64_t a = (uint64_t)from;  // (the same in all lanes)
-    const uint64_t base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)a);
-    lds = __builtin_amdgcn_readfirstlane(lds);
+// One such copy: 16 bytes a lane from base + off to 1024 bytes of LDS.  Written out, because the compiler takes
+// any LDS read behind its own form of it as one that has to wait for all copies; the waits are the kernel's (ready()).
+__device__ __forceinline__ void copy_to_lds(const f16* base, uint32_t off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base));
 }
+__device__ __forceinline__ const f16* uniform(const f16* p) {  // (the same in all lanes: to scalar registers)
+    const uint64_t a = (uint64_t)p;
+    return (const f16*)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)a));
+}
 
+// A K-step's copies are dealt to the four waves in turn, so that copy u of a wave belongs to an array that is known when this is
+// compiled, and its rows to one of OFFS byte offsets that stay the same throughout: what is left to do is a scalar addition each.
+// (With the addresses made from the copy's number a step of 108 products spent as long on 400 scalar instructions.)
 struct Sources {  // the first rows of a tile's operands: hi of L, hi of R, lo of L, lo of R
     const f16 *a, *b, *c, *d;
 };
-template <int TILE, int BK, int ARRAYS>
-__device__ __forceinline__ void stage(uint32_t lds, const Sources& src, int ld, int k0) {
-    constexpr int CPR = BK / 8, RPI = 64 / CPR, EACH = ARRAYS * TILE / RPI / 4;  // chunks to a row, rows to an instruction, instructions to a wave
-    const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-    const int row = lane / CPR, chunk = place<BK>(row, lane % CPR);
-    const uint32_t off = (uint32_t)(row * ld + chunk * 8) * 2;
+template <int TILE, int BK>
+constexpr int offsets_of() {
+    return TILE * BK / 512 / 4;
+}
+template <int TILE, int BK>
+__device__ __forceinline__ void offsets(int ld, uint32_t (&off)[offsets_of<TILE, BK>()]) {
+    constexpr int CPR = BK / 8, RPI = 64 / CPR;  // chunks to a row, rows to a copy
+    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, row = lane / CPR, chunk = place<BK>(row, lane % CPR);
 #pragma unroll
-    for (int u = 0; u < EACH; u++) {
-        const int t = wave * EACH + u, array = t / (TILE / RPI), part = t % (TILE / RPI);
-        const f16* s = array == 0 ? src.a : array == 1 ? src.b : array == 2 ? src.c : src.d;
-        copy_to_lds(s + (int64_t)part * RPI * ld + k0, off, lds + t * 1024);
+    for (int u = 0; u < offsets_of<TILE, BK>(); u++) off[u] = (uint32_t)(((u * 4 + wave) * RPI + row) * ld + chunk * 8) * 2;
+}
+// copies [from, to) of a K-step
+template <int TILE, int BK>
+__device__ __forceinline__ void stage(uint32_t lds, const Sources& src, const uint32_t (&off)[offsets_of<TILE, BK>()], int k0, int from, int to) {
+    constexpr int OFFS = offsets_of<TILE, BK>();
+#pragma unroll
+    for (int u = from; u < to; u++) {
+        const int array = u / OFFS;
+        copy_to_lds((array == 0 ? src.a : array == 1 ? src.b : array == 2 ? src.c : src.d) + k0, off[u % OFFS], lds + u * 4096);
     }
 }
 
-// fragments of one operand: NF blocks of 16 rows, 32 halves of K
-template <int BK, int NF>
-__device__ __forceinline__ void fragments(const f16* lds, int first, int kk, half8 (&f)[NF]) {
-    const int lane = threadIdx.x % WAVE;
-#pragma unroll
-    for (int x = 0; x < NF; x++) {
-        const int row = first + x * 16 + lane % 16;
-        f[x] = *(const half8*)&lds[row * BK + place<BK>(row, kk * 4 + lane / 16) * 8];
-    }
+// fragment x of one operand: 16 rows, 32 halves of K
+template <int BK>
+__device__ __forceinline__ half8 fragment(const f16* lds, int first, int kk, int x) {
+    const int lane = threadIdx.x % WAVE, row = first + x * 16 + lane % 16;
+    return *(const half8*)&lds[row * BK + place<BK>(row, kk * 4 + lane / 16) * 8];
 }
-// all products of two operands' fragments, with `READS` LDS reads of the next ones spread between them
-template <int NF, int READS>
-__device__ __forceinline__ void products(const half8 (&l)[NF], const half8 (&r)[NF], float4_ (&acc)[NF][NF]) {
+// All products of two operands' fragments, NF at a time: before each of these, slot(n) asks for what is needed later -- reads of LDS
+// and copies to it, a few at a time, so that the matrix unit always has products to work on while they are served.
+template <bool BY_ROW, int NF, class F>
+__device__ __forceinline__ void products(const half8 (&l)[NF], const half8 (&r)[NF], float4_ (&acc)[NF][NF], F slot) {
 #pragma unroll
-    for (int x = 0; x < NF; x++)
+    for (int n = 0; n < NF; n++) {
+        slot(n);
 #pragma unroll
-        for (int y = 0; y < NF; y++) acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[x], r[y], acc[x][y], 0, 0, 0);
-    constexpr int GAP = NF * NF / (READS + 1) > 0 ? NF * NF / (READS + 1) : 1;
-#pragma unroll
-    for (int k = 0; k < READS; k++) {
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // a read ...
-        __builtin_amdgcn_sched_group_barrier(0x008, GAP, 0);  // ... and some products
+        for (int m = 0; m < NF; m++) {
+            const int x = BY_ROW ? n : m, y = BY_ROW ? m : n;
+            acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[x], r[y], acc[x][y], 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 
@@ -220,7 +229,9 @@ template <class T, int WHAT, int PARTS, int TILE, int STAGES>
 __global__ __launch_bounds__(256, TILE <= 128 && STAGES * TILE <= 256 ? 2 : 1) void product_kernel(Product first, Product second, int batch) {
     constexpr int BK = PARTS == 1 ? 64 : 32, ARRAYS = PARTS == 1 ? 2 : PARTS + 1, NF = TILE / 32, ARRAY = TILE * BK;
     constexpr int EACH = ARRAYS * ARRAY / 512 / 4;  // copies of a stage to a wave
-    __shared__ __attribute__((aligned(1024))) f16 s0[ARRAYS * ARRAY], s1[ARRAYS * ARRAY], s2[STAGES > 2 ? ARRAYS * ARRAY : 8], s3[STAGES > 3 ? ARRAYS * ARRAY : 8];
+    constexpr int LINE = TILE + 4;  // of the 32-bit result in LDS
+    constexpr int STAGED = STAGES * ARRAYS * ARRAY * 2, RESULT = TILE * LINE * 4;
+    __shared__ __attribute__((aligned(1024))) char pool[STAGED > RESULT ? STAGED : RESULT];
     const Product& p = (int)blockIdx.z < batch ? first : second;
     const int64_t b = blockIdx.z % batch;
     const Place at = place_of(blockIdx.x, gridDim.x, (p.rows + TILE - 1) / TILE, (p.cols + TILE - 1) / TILE, WHAT == SYM || WHAT == POLY);
@@ -228,7 +239,9 @@ __global__ __launch_bounds__(256, TILE <= 128 && STAGES * TILE <= 256 ? 2 : 1) v
     const int tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
     const int wi = (wave / 2) * (TILE / 2), wj = (wave % 2) * (TILE / 2);
     const int64_t l_first = b * p.l_batch + (int64_t)ti * TILE * p.ld, r_first = b * p.r_batch + (int64_t)tj * TILE * p.ld;
-    const Sources src = {p.l.hi + l_first, p.r.hi + r_first, p.l.lo + l_first, p.r.lo + r_first};
+    const Sources src = {uniform(p.l.hi + l_first), uniform(p.r.hi + r_first), uniform(p.l.lo + l_first), uniform(p.r.lo + r_first)};
+    uint32_t off[offsets_of<TILE, BK>()];
+    offsets<TILE, BK>(p.ld, off);
     float4_ acc[NF][NF];
 #pragma unroll
     for (int x = 0; x < NF; x++)
@@ -244,92 +257,160 @@ __global__ __launch_bounds__(256, TILE <= 128 && STAGES * TILE <= 256 ? 2 : 1) v
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    auto ask = [&](const f16* buf, int k) {  // (behind the last step the first is copied once more: the count of copies stays)
-        stage<TILE, BK, ARRAYS>((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)buf, src, p.ld, k < steps ? k * BK : 0);
+    // A stage's copies are spread over the products that follow its becoming free: SLOTS groups of NF of them, the last NF groups of a
+    // step and, where there are stages enough, all of the next step's before it waits.
+    constexpr bool SPREAD = STAGES > 2;
+    constexpr int SLOTS = (!SPREAD ? 1 : PARTS == 3 ? 3 : 2) * NF;
+    const uint32_t pool_at = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)pool;
+    auto ask = [&](int buf, int k, int from, int to) {  // (behind the last step that one is copied once more: the count of copies stays)
+        const uint32_t lds = __builtin_amdgcn_readfirstlane(pool_at + (uint32_t)wave * 1024) + buf * (ARRAYS * ARRAY * 2);
+        stage<TILE, BK>(lds, src, off, (k < steps ? k : steps - 1) * BK, from * EACH / SLOTS, to * EACH / SLOTS);
     };
     half8 l[NF], r[NF], u[NF], v[NF];  // the step's first fragments; those that follow them
-    auto step = [&](f16* now, f16* next, f16* fill, int k) {
+    constexpr int READS = 2 * NF;      // of the next step's first fragments, of R before L
+    constexpr int EARLY = (READS + NF - 2) / (NF - 1);
+    auto step = [&](int h, int k) {
+        const f16* now = (const f16*)pool + h * ARRAYS * ARRAY;
+        const f16* next = (const f16*)pool + (h + 1) % STAGES * ARRAYS * ARRAY;
+        const int prev = (h + STAGES - 1) % STAGES;
+        half8 w[NF];
+        auto lead = [&](int n) {  // the next step's first fragments
+            ask(h, k + STAGES, n, n + 1);
+#pragma unroll
+            for (int q = n * EARLY; q < READS && q < (n + 1) * EARLY; q++) {
+                if (q < NF)
+                    w[q] = fragment<BK>(next + ARRAY, wj, 0, q);
+                else
+                    l[q - NF] = fragment<BK>(next, wi, 0, q - NF);
+            }
+        };
         if (PARTS == 1) {
-            fragments<BK, NF>(now, wi, 1, u);
-            fragments<BK, NF>(now + ARRAY, wj, 1, v);
-            products<NF, 2 * NF>(l, r, acc);
+            products<true>(l, r, acc, [&](int n) {
+                if (SPREAD) ask(prev, k + STAGES - 1, NF + n, NF + n + 1);
+#pragma unroll
+                for (int q = n * EARLY; q < READS && q < (n + 1) * EARLY; q++) {
+                    if (q < NF)
+                        v[q] = fragment<BK>(now + ARRAY, wj, 1, q);
+                    else
+                        u[q - NF] = fragment<BK>(now, wi, 1, q - NF);
+                }
+            });
             ready();
-            ask(fill, k + STAGES);
-            fragments<BK, NF>(next, wi, 0, l);
-            fragments<BK, NF>(next + ARRAY, wj, 0, r);
-            products<NF, 2 * NF>(u, v, acc);
+            products<true>(u, v, acc, lead);
         } else {
             if (PARTS == 3) {
-                fragments<BK, NF>(now + 3 * ARRAY, wj, 0, v);  // lo of R
-                products<NF, NF>(l, r, acc);                   // hi hi
-                fragments<BK, NF>(now + 2 * ARRAY, wi, 0, u);  // lo of L
-                products<NF, NF>(l, v, acc);                   // hi lo
+                products<true>(l, r, acc, [&](int n) {   // hi hi
+                    if (SPREAD) ask(prev, k + STAGES - 1, NF + n, NF + n + 1);
+#pragma unroll
+                    for (int q = n * 2; q < NF && q < n * 2 + 2; q++) v[q] = fragment<BK>(now + 3 * ARRAY, wj, 0, q);  // lo of R
+                });
+                products<false>(l, v, acc, [&](int n) {  // hi lo
+                    if (SPREAD) ask(prev, k + STAGES - 1, 2 * NF + n, 2 * NF + n + 1);
+#pragma unroll
+                    for (int q = n * 2; q < NF && q < n * 2 + 2; q++) u[q] = fragment<BK>(now + 2 * ARRAY, wi, 0, q);  // lo of L
+                });
             } else {
-                fragments<BK, NF>(now + 2 * ARRAY, wi, 0, u);
-                products<NF, NF>(l, r, acc);
+                products<true>(l, r, acc, [&](int n) {
+                    if (SPREAD) ask(prev, k + STAGES - 1, NF + n, NF + n + 1);
+#pragma unroll
+                    for (int q = n * 2; q < NF && q < n * 2 + 2; q++) u[q] = fragment<BK>(now + 2 * ARRAY, wi, 0, q);
+                });
             }
             ready();
-            ask(fill, k + STAGES);
-            fragments<BK, NF>(next, wi, 0, l);
-            fragments<BK, NF>(next + ARRAY, wj, 0, v);
-            products<NF, 2 * NF>(u, r, acc);                   // lo hi
-#pragma unroll
-            for (int x = 0; x < NF; x++) r[x] = v[x];
+            products<true>(u, r, acc, lead);             // lo hi
         }
-    };
-    f16* const buf[4] = {s0, s1, s2, s3};
 #pragma unroll
-    for (int k = 0; k < STAGES; k++) ask(buf[k], k);
+        for (int x = 0; x < NF; x++) r[x] = w[x];
+    };
+#pragma unroll
+    for (int k = 0; k < STAGES - 1; k++) ask(k, k, 0, SLOTS);
+    ask(STAGES - 1, STAGES - 1, 0, NF);
     {
-        constexpr int out = EACH * (STAGES - 1);
+        constexpr int out = EACH * (STAGES - 2) + NF * EACH / SLOTS;
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_waitcnt(0x0f70 | (out & 15) | ((out >> 4) << 14));
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     }
-    fragments<BK, NF>(s0, wi, 0, l);
-    fragments<BK, NF>(s0 + ARRAY, wj, 0, r);
+#pragma unroll
+    for (int x = 0; x < NF; x++) l[x] = fragment<BK>((const f16*)pool, wi, 0, x), r[x] = fragment<BK>((const f16*)pool + ARRAY, wj, 0, x);
     for (int k = 0; k < steps; k += STAGES) {
 #pragma unroll
         for (int h = 0; h < STAGES; h++)
-            if (k + h < steps) step(buf[h], buf[(h + 1) % STAGES], buf[h], k + h);
+            if (k + h < steps) step(h, k + h);
     }
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // the copies behind the last step: none may outlive the workgroup
-    float scale = p.scale;
-    if (p.inv_power) scale *= p.inv_power == 1 ? p.inv[b] : p.inv[b] * p.inv[b];
-    // a lane holds rows i .. i+3 of column j of each 16 x 16 block
+    // The result goes through LDS, in 32 bits: a lane has 4 adjacent rows of a column, and what is stored are rows, of C and of
+    // its transpose, 16 bytes a lane.  (Stored from the registers, 2 bytes a lane, the code for it alone -- 20 KB in a straight
+    // line, fetched once -- took 14 us for a tile of 192.)  A column's rows are turned by 16 in every other 8 columns: the reads
+    // across columns then find other banks.
+    __builtin_amdgcn_s_waitcnt(0x0070);  // the copies behind the last step, and this wave's LDS reads
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    float* const res = (float*)pool;
+    auto spot = [](int i, int j) { return j * LINE + (i + 16 * (j >> 3 & 1)) % TILE; };
 #pragma unroll
     for (int x = 0; x < NF; x++)
 #pragma unroll
-        for (int y = 0; y < NF; y++) {
-            const int i = ti * TILE + wi + x * 16 + (lane / 16) * 4, j = tj * TILE + wj + y * 16 + lane % 16;
-            if (WHAT != LAST && (i >= p.rows || j >= p.cols)) continue;
-            half4 hi, lo, s_hi, s_lo;
+        for (int y = 0; y < NF; y++) *(float4_*)&res[spot(wi + x * 16 + (lane / 16) * 4, wj + y * 16 + lane % 16)] = acc[x][y];
+    __syncthreads();
+    float scale = p.scale;
+    if (p.inv_power) scale *= p.inv_power == 1 ? p.inv[b] : p.inv[b] * p.inv[b];
+    // 8 adjacent values of one row of C (or of its transpose): row `first`, columns `second` ...
+    auto emit = [&](const float (&v)[8], int first, int second, bool transposed) {
+        if constexpr (WHAT == LAST) {
+            const int rows = transposed ? p.n : p.m, cols = transposed ? p.m : p.n;
+            if (first >= rows || second >= cols) return;
+            T* o = (T*)p.out + b * (int64_t)p.m * p.n + (int64_t)first * cols + second;
+            Pack<T, 8> w;
+#pragma unroll
+            for (int e = 0; e < 8; e++) w.v[e] = (T)(v[e] * scale);
+            if (second + 8 <= cols)
+                *(Pack<T, 8>*)o = w;
+            else
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (second + e < cols) o[e] = w.v[e];
+        } else {
+            if (first >= (transposed ? p.cols : p.rows) || second >= (transposed ? p.rows : p.cols)) return;
+            half8 hi, lo, s_hi, s_lo;
             if (WHAT == POLY) {  // (S is symmetric)
-                const int64_t at = b * p.l_batch + (int64_t)j * p.ld + i;
-                s_hi = *(const half4*)(p.l.hi + at), s_lo = *(const half4*)(p.l.lo + at);
+                const int64_t from = b * p.l_batch + (int64_t)first * p.ld + second;
+                s_hi = *(const half8*)(p.l.hi + from), s_lo = *(const half8*)(p.l.lo + from);
             }
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                float v = acc[x][y][e] * scale;
+            for (int e = 0; e < 8; e++) {
+                float w = v[e] * scale;
                 if (WHAT == POLY) {
-                    v += p.b * ((float)s_hi[e] + (float)s_lo[e]);
-                    if (i + e == j && j < p.m) v += p.a;
+                    w += p.b * ((float)s_hi[e] + (float)s_lo[e]);
+                    if (first == second + e && first < p.m) w += p.a;
                 }
-                if (WHAT == LAST) {
-                    if (i + e < p.m && j < p.n) ((T*)p.out)[b * (int64_t)p.m * p.n + (p.tall ? (int64_t)j * p.m + i + e : (int64_t)(i + e) * p.n + j)] = (T)v;
-                } else {
-                    const Halves h = split(v);
-                    hi[e] = h.hi, lo[e] = h.lo;
-                    const int64_t o = b * p.o_batch + (int64_t)(i + e) * p.o_ld + j;
-                    p.o.hi[o] = h.hi, p.o.lo[o] = h.lo;
-                }
+                const Halves h = split(w);
+                hi[e] = h.hi, lo[e] = h.lo;
             }
-            if (WHAT == STEP || (WHAT != LAST && ti != tj)) {
-                const int64_t t = b * p.o_batch + (int64_t)j * p.t_ld + i;
-                *(half4*)(p.t.hi + t) = hi, *(half4*)(p.t.lo + t) = lo;
-            }
+            const int64_t to = b * p.o_batch + (int64_t)first * (transposed ? p.t_ld : p.o_ld) + second;
+            *(half8*)((transposed ? p.t.hi : p.o.hi) + to) = hi;
+            *(half8*)((transposed ? p.t.lo : p.o.lo) + to) = lo;
         }
+    };
+    if (WHAT == STEP || (WHAT == LAST && p.tall) || ((WHAT == SYM || WHAT == POLY) && ti != tj)) {
+#pragma unroll 2
+        for (int k = tid; k < TILE * TILE / 8; k += 256) {
+            const int j = k / (TILE / 8), i = k % (TILE / 8) * 8;
+            float v[8];
+            *(float4_*)v = *(const float4_*)&res[spot(i, j)], *(float4_*)(v + 4) = *(const float4_*)&res[spot(i, j) + 4];
+            emit(v, tj * TILE + j, ti * TILE + i, true);
+        }
+    }
+    if (WHAT != LAST || !p.tall) {
+#pragma unroll 2
+        for (int k = tid; k < TILE * TILE / 8; k += 256) {
+            const int g = k / WAVE, i = g % (TILE / 16) * 16 + lane % 16, j = g / (TILE / 16) * 32 + lane / 16 * 8;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = res[spot(i, j + e)];
+            emit(v, ti * TILE + i, tj * TILE + j, false);
+        }
+    }
 }
 
 // ------------------------------------------------------------------------------------ launches
@@ -404,16 +485,18 @@ static void launch_tiles(const Product& p, const Product* second, int batch, hip
     const int tiles = WHAT == SYM || WHAT == POLY ? rows * (rows + 1) / 2 : rows * cols;
     product_kernel<T, WHAT, PARTS, TILE, STAGES><<<dim3(tiles, 1, second ? 2 * batch : batch), 256, 0, s>>>(p, second ? *second : p, batch);
 }
-// The tile: what the compute unit with the most of them takes, from the time of a K-step of each (three products, all units
-// busy, measured at 4000 x 4100): 64: 0.35 us, 128: 0.95, 192: 1.55.
+// The tile: the one with which the compute unit that has the most of them is done first.  What a tile takes, in us, measured with
+// three products a K-step at 4000 x 4100 (all units busy) and 128 x 256 (a few steps): 64: 0.31 a step and 1.5 beside, 128: 0.72 and 4,
+// 192: 1.32 and 8.  (64 and 128 in two stages: two workgroups a unit.)
 template <class T, int WHAT, int PARTS>
 static void launch_product(const Product& p, const Product* second, int batch, hipStream_t s) {
+    const double steps = p.k / 32 * (PARTS / 3.0);
     auto rounds = [&](int tile) {
         const int64_t rows = (p.rows + tile - 1) / tile, cols = (p.cols + tile - 1) / tile;
         const int64_t tiles = (WHAT == SYM || WHAT == POLY ? rows * (rows + 1) / 2 : rows * cols) * batch * (second ? 2 : 1);
         return (tiles + 255) / 256;
     };
-    const double t64 = 0.35 * rounds(64), t128 = 0.95 * rounds(128), t192 = 1.55 * rounds(192);
+    const double t64 = rounds(64) * (0.31 * steps + 1.5), t128 = rounds(128) * (0.72 * steps + 4), t192 = rounds(192) * (1.32 * steps + 8);
     if (t192 < t128 && t192 < t64)
         launch_tiles<T, WHAT, PARTS, 192, 3>(p, second, batch, s);
     else if (t128 < t64 && rounds(128) == 1)
@@ -482,10 +565,11 @@ static void launch_orthogonalize(const Plan& q, const void* g, void* out, const 
     for (int k = 0; k < q.gram; k++) {
         const int now = k & 1;
         const bool more = k + 1 < q.gram;
-        if (k == 0) launch_product<float, POLY, 3>(poly(f.s[0], f.q[0], q.sq), nullptr, q.batch, s);  // Q = P
-        if (k || more) launch_product<float, POLY, 3>(poly(f.s[now], f.p, q.sp), nullptr, q.batch, s);
-        Product pp = square(q, f.p, f.p, f.t), qp = square(q, f.q[now ^ 1], f.p, f.q[now]);
-        pp.scale = (float)(q.st / (q.sp * q.sp)), qp.scale = (float)(1 / q.sp);
+        const Split step = k ? f.p : f.q[0];  // (Q = P at first)
+        const double step_scale = k ? q.sp : q.sq;
+        launch_product<float, POLY, 3>(poly(f.s[now], step, step_scale), nullptr, q.batch, s);
+        Product pp = square(q, step, step, f.t), qp = square(q, f.q[now ^ 1], f.p, f.q[now]);
+        pp.scale = (float)(q.st / (step_scale * step_scale)), qp.scale = (float)(1 / q.sp);
         if (more) {
             launch_product<float, SYM, 3>(pp, k ? &qp : nullptr, q.batch, s);
             Product next = square(q, f.s[now], f.t, f.s[now ^ 1]);
