@@ -174,7 +174,7 @@ __device__ __forceinline__ const f16* uniform(const f16* p) {  // (the same in a
     return (const f16*)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)a));
 }
 
-// A K-step's copies are dealt to the four waves in turn, so that copy u of a wave belongs to an array that is known when this is
+// A K-step's copies are dealt to four waves in turn (of eight, each four have half of the arrays), so that copy u of a wave belongs to an array that is known when this is
 // compiled, and its rows to one of OFFS byte offsets that stay the same throughout: what is left to do is a scalar addition each.
 // (With the addresses made from the copy's number a step of 108 products spent as long on 400 scalar instructions.)
 struct Sources {  // the first rows of a tile's operands: hi of L, hi of R, lo of L, lo of R
@@ -187,7 +187,7 @@ constexpr int offsets_of() {
 template <int TILE, int BK>
 __device__ __forceinline__ void offsets(int ld, uint32_t (&off)[offsets_of<TILE, BK>()]) {
     constexpr int CPR = BK / 8, RPI = 64 / CPR;  // chunks to a row, rows to a copy
-    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, row = lane / CPR, chunk = place<BK>(row, lane % CPR);
+    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE % 4, row = lane / CPR, chunk = place<BK>(row, lane % CPR);
 #pragma unroll
     for (int u = 0; u < offsets_of<TILE, BK>(); u++) off[u] = (uint32_t)(((u * 4 + wave) * RPI + row) * ld + chunk * 8) * 2;
 }
@@ -208,27 +208,26 @@ __device__ __forceinline__ half8 fragment(const f16* lds, int first, int kk, int
     const int lane = threadIdx.x % WAVE, row = first + x * 16 + lane % 16;
     return *(const half8*)&lds[row * BK + place<BK>(row, kk * 4 + lane / 16) * 8];
 }
-// All products of two operands' fragments, NF at a time: before each of these, slot(n) asks for what is needed later -- reads of LDS
+// All products of two operands' fragments, a column at a time: before each, slot(n) asks for what is needed later -- reads of LDS
 // and copies to it, a few at a time, so that the matrix unit always has products to work on while they are served.
-template <bool BY_ROW, int NF, class F>
-__device__ __forceinline__ void products(const half8 (&l)[NF], const half8 (&r)[NF], float4_ (&acc)[NF][NF], F slot) {
+template <int NI, int NJ, class F>
+__device__ __forceinline__ void products(const half8 (&l)[NI], const half8 (&r)[NJ], float4_ (&acc)[NI][NJ], F slot) {
 #pragma unroll
-    for (int n = 0; n < NF; n++) {
+    for (int n = 0; n < NJ; n++) {
         slot(n);
 #pragma unroll
-        for (int m = 0; m < NF; m++) {
-            const int x = BY_ROW ? n : m, y = BY_ROW ? m : n;
-            acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[x], r[y], acc[x][y], 0, 0, 0);
-        }
+        for (int x = 0; x < NI; x++) acc[x][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[x], r[n], acc[x][n], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
     }
 }
 
 // The second product of a launch, if there is one, is that of the workgroups with the higher numbers along z.
-template <class T, int WHAT, int PARTS, int TILE, int STAGES>
-__global__ __launch_bounds__(256, TILE <= 128 && STAGES * TILE <= 256 ? 2 : 1) void product_kernel(Product first, Product second, int batch) {
-    constexpr int BK = PARTS == 1 ? 64 : 32, ARRAYS = PARTS == 1 ? 2 : PARTS + 1, NF = TILE / 32, ARRAY = TILE * BK;
-    constexpr int EACH = ARRAYS * ARRAY / 512 / 4;  // copies of a stage to a wave
+template <class T, int WHAT, int PARTS, int TILE, int STAGES, int WAVES>
+__global__ __launch_bounds__(WAVES * WAVE, TILE <= 128 && STAGES * TILE <= 256 ? 2 : WAVES / 4) void product_kernel(Product first, Product second, int batch) {
+    constexpr int BK = PARTS == 1 ? 64 : 32, ARRAYS = PARTS == 1 ? 2 : PARTS + 1, ARRAY = TILE * BK;
+    constexpr int NI = TILE / 32, NJ = TILE / 16 / (WAVES / 2);  // a wave's blocks: the waves lie 2 x WAVES / 2
+    constexpr int TEAMS = WAVES / 4, EACH = ARRAYS * ARRAY / 512 / WAVES;  // four waves copy every TEAMS-th part of the arrays; copies of a stage to a wave
+    static_assert(ARRAYS % TEAMS == 0, "a team's arrays");
     constexpr int LINE = TILE + 4;  // of the 32-bit result in LDS
     constexpr int STAGED = STAGES * ARRAYS * ARRAY * 2, RESULT = TILE * LINE * 4;
     __shared__ __attribute__((aligned(1024))) char pool[STAGED > RESULT ? STAGED : RESULT];
@@ -237,16 +236,18 @@ __global__ __launch_bounds__(256, TILE <= 128 && STAGES * TILE <= 256 ? 2 : 1) v
     const Place at = place_of(blockIdx.x, gridDim.x, (p.rows + TILE - 1) / TILE, (p.cols + TILE - 1) / TILE, WHAT == SYM || WHAT == POLY);
     const int ti = at.i, tj = at.j;
     const int tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
-    const int wi = (wave / 2) * (TILE / 2), wj = (wave % 2) * (TILE / 2);
+    const int wi = wave / (WAVES / 2) * (TILE / 2), wj = wave % (WAVES / 2) * (NJ * 16);
     const int64_t l_first = b * p.l_batch + (int64_t)ti * TILE * p.ld, r_first = b * p.r_batch + (int64_t)tj * TILE * p.ld;
-    const Sources src = {uniform(p.l.hi + l_first), uniform(p.r.hi + r_first), uniform(p.l.lo + l_first), uniform(p.r.lo + r_first)};
+    const bool later = TEAMS == 2 && wave >= 4;  // the second team: the second half of the arrays
+    const Sources src = {uniform(!later ? p.l.hi + l_first : ARRAYS == 2 ? p.r.hi + r_first : p.l.lo + l_first),
+                         uniform(!later ? p.r.hi + r_first : p.r.lo + r_first), uniform(p.l.lo + l_first), uniform(p.r.lo + r_first)};
     uint32_t off[offsets_of<TILE, BK>()];
     offsets<TILE, BK>(p.ld, off);
-    float4_ acc[NF][NF];
+    float4_ acc[NI][NJ], low[NI][NJ];  // of hi hi, and (three parts) of the others, 2^-11 of it: added to it one by one they would be cut off
 #pragma unroll
-    for (int x = 0; x < NF; x++)
+    for (int x = 0; x < NI; x++)
 #pragma unroll
-        for (int y = 0; y < NF; y++) acc[x][y] = float4_{0, 0, 0, 0};
+        for (int y = 0; y < NJ; y++) acc[x][y] = low[x][y] = float4_{0, 0, 0, 0};
     // The copies of STAGES - 1 K-steps are under way while one is multiplied.  ready(): the oldest stage's copies of this wave
     // have arrived (the younger ones may still be out), then everybody's have, and nobody reads the stage that is filled next.
     const int steps = p.k / BK;
@@ -257,83 +258,78 @@ __global__ __launch_bounds__(256, TILE <= 128 && STAGES * TILE <= 256 ? 2 : 1) v
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    // A stage's copies are spread over the products that follow its becoming free: SLOTS groups of NF of them, the last NF groups of a
+    // A stage's copies are spread over the products that follow its becoming free: SLOTS columns of them, the last NJ of a
     // step and, where there are stages enough, all of the next step's before it waits.
     constexpr bool SPREAD = STAGES > 2;
-    constexpr int SLOTS = (!SPREAD ? 1 : PARTS == 3 ? 3 : 2) * NF;
+    constexpr int SLOTS = (!SPREAD ? 1 : PARTS == 3 ? 3 : 2) * NJ;
     const uint32_t pool_at = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)pool;
     auto ask = [&](int buf, int k, int from, int to) {  // (behind the last step that one is copied once more: the count of copies stays)
-        const uint32_t lds = __builtin_amdgcn_readfirstlane(pool_at + (uint32_t)wave * 1024) + buf * (ARRAYS * ARRAY * 2);
+        const uint32_t lds = __builtin_amdgcn_readfirstlane(pool_at + (uint32_t)(wave % 4 * 1024 + wave / 4 * (ARRAYS / TEAMS * ARRAY * 2))) + buf * (ARRAYS * ARRAY * 2);
         stage<TILE, BK>(lds, src, off, (k < steps ? k : steps - 1) * BK, from * EACH / SLOTS, to * EACH / SLOTS);
     };
-    half8 l[NF], r[NF], u[NF], v[NF];  // the step's first fragments; those that follow them
-    constexpr int READS = 2 * NF;      // of the next step's first fragments, of R before L
-    constexpr int EARLY = (READS + NF - 2) / (NF - 1);
+    // The products go column by column: a fragment of R is done with then, and the next step's takes its registers.
+    constexpr int LOT = (NI + NJ - 1) / NJ + (NJ > 3);  // fragments of L to a column, so that the last come before they are needed
+    half8 l[NI], r[NJ], u[NI], v[NJ];  // the step's first fragments; those that follow them
     auto step = [&](int h, int k) {
         const f16* now = (const f16*)pool + h * ARRAYS * ARRAY;
         const f16* next = (const f16*)pool + (h + 1) % STAGES * ARRAYS * ARRAY;
         const int prev = (h + STAGES - 1) % STAGES;
-        half8 w[NF];
-        auto lead = [&](int n) {  // the next step's first fragments
-            ask(h, k + STAGES, n, n + 1);
-#pragma unroll
-            for (int q = n * EARLY; q < READS && q < (n + 1) * EARLY; q++) {
-                if (q < NF)
-                    w[q] = fragment<BK>(next + ARRAY, wj, 0, q);
-                else
-                    l[q - NF] = fragment<BK>(next, wi, 0, q - NF);
-            }
-        };
         if (PARTS == 1) {
-            products<true>(l, r, acc, [&](int n) {
-                if (SPREAD) ask(prev, k + STAGES - 1, NF + n, NF + n + 1);
+            products(l, r, acc, [&](int n) {
+                if (SPREAD) ask(prev, k + STAGES - 1, NJ + n, NJ + n + 1);
 #pragma unroll
-                for (int q = n * EARLY; q < READS && q < (n + 1) * EARLY; q++) {
-                    if (q < NF)
-                        v[q] = fragment<BK>(now + ARRAY, wj, 1, q);
-                    else
-                        u[q - NF] = fragment<BK>(now, wi, 1, q - NF);
-                }
+                for (int q = n * LOT; q < NI && q < n * LOT + LOT; q++) u[q] = fragment<BK>(now, wi, 1, q);
+                v[n] = fragment<BK>(now + ARRAY, wj, 1, n);
             });
             ready();
-            products<true>(u, v, acc, lead);
+            products(u, v, acc, [&](int n) {
+                ask(h, k + STAGES, n, n + 1);
+#pragma unroll
+                for (int q = n * LOT; q < NI && q < n * LOT + LOT; q++) l[q] = fragment<BK>(next, wi, 0, q);
+                r[n] = fragment<BK>(next + ARRAY, wj, 0, n);
+            });
         } else {
             if (PARTS == 3) {
-                products<true>(l, r, acc, [&](int n) {   // hi hi
-                    if (SPREAD) ask(prev, k + STAGES - 1, NF + n, NF + n + 1);
-#pragma unroll
-                    for (int q = n * 2; q < NF && q < n * 2 + 2; q++) v[q] = fragment<BK>(now + 3 * ARRAY, wj, 0, q);  // lo of R
+                products(l, r, acc, [&](int n) {  // hi hi
+                    if (SPREAD) ask(prev, k + STAGES - 1, NJ + n, NJ + n + 1);
+                    v[n] = fragment<BK>(now + 3 * ARRAY, wj, 0, n);  // lo of R
                 });
-                products<false>(l, v, acc, [&](int n) {  // hi lo
-                    if (SPREAD) ask(prev, k + STAGES - 1, 2 * NF + n, 2 * NF + n + 1);
+                products(l, v, low, [&](int n) {  // hi lo
+                    if (SPREAD) ask(prev, k + STAGES - 1, 2 * NJ + n, 2 * NJ + n + 1);
 #pragma unroll
-                    for (int q = n * 2; q < NF && q < n * 2 + 2; q++) u[q] = fragment<BK>(now + 2 * ARRAY, wi, 0, q);  // lo of L
+                    for (int q = n * LOT; q < NI && q < n * LOT + LOT; q++) u[q] = fragment<BK>(now + 2 * ARRAY, wi, 0, q);  // lo of L
                 });
             } else {
-                products<true>(l, r, acc, [&](int n) {
-                    if (SPREAD) ask(prev, k + STAGES - 1, NF + n, NF + n + 1);
+                products(l, r, acc, [&](int n) {
+                    if (SPREAD) ask(prev, k + STAGES - 1, NJ + n, NJ + n + 1);
 #pragma unroll
-                    for (int q = n * 2; q < NF && q < n * 2 + 2; q++) u[q] = fragment<BK>(now + 2 * ARRAY, wi, 0, q);
+                    for (int q = n * LOT; q < NI && q < n * LOT + LOT; q++) u[q] = fragment<BK>(now + 2 * ARRAY, wi, 0, q);
                 });
             }
             ready();
-            products<true>(u, r, acc, lead);             // lo hi
-        }
+            products(u, r, PARTS == 3 ? low : acc, [&](int n) {  // lo hi
+                ask(h, k + STAGES, n, n + 1);
 #pragma unroll
-        for (int x = 0; x < NF; x++) r[x] = w[x];
+                for (int q = n * LOT; q < NI && q < n * LOT + LOT; q++) l[q] = fragment<BK>(next, wi, 0, q);
+                if (n) r[n - 1] = fragment<BK>(next + ARRAY, wj, 0, n - 1);
+            });
+            r[NJ - 1] = fragment<BK>(next + ARRAY, wj, 0, NJ - 1);
+        }
     };
 #pragma unroll
     for (int k = 0; k < STAGES - 1; k++) ask(k, k, 0, SLOTS);
-    ask(STAGES - 1, STAGES - 1, 0, NF);
+    ask(STAGES - 1, STAGES - 1, 0, NJ);
     {
-        constexpr int out = EACH * (STAGES - 2) + NF * EACH / SLOTS;
+        constexpr int out = EACH * (STAGES - 2) + NJ * EACH / SLOTS;
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_waitcnt(0x0f70 | (out & 15) | ((out >> 4) << 14));
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     }
 #pragma unroll
-    for (int x = 0; x < NF; x++) l[x] = fragment<BK>((const f16*)pool, wi, 0, x), r[x] = fragment<BK>((const f16*)pool + ARRAY, wj, 0, x);
+    for (int x = 0; x < NI; x++) l[x] = fragment<BK>((const f16*)pool, wi, 0, x);
+#pragma unroll
+    for (int y = 0; y < NJ; y++) r[y] = fragment<BK>((const f16*)pool + ARRAY, wj, 0, y);
     for (int k = 0; k < steps; k += STAGES) {
 #pragma unroll
         for (int h = 0; h < STAGES; h++)
@@ -349,9 +345,9 @@ __global__ __launch_bounds__(256, TILE <= 128 && STAGES * TILE <= 256 ? 2 : 1) v
     float* const res = (float*)pool;
     auto spot = [](int i, int j) { return j * LINE + (i + 16 * (j >> 3 & 1)) % TILE; };
 #pragma unroll
-    for (int x = 0; x < NF; x++)
+    for (int x = 0; x < NI; x++)
 #pragma unroll
-        for (int y = 0; y < NF; y++) *(float4_*)&res[spot(wi + x * 16 + (lane / 16) * 4, wj + y * 16 + lane % 16)] = acc[x][y];
+        for (int y = 0; y < NJ; y++) *(float4_*)&res[spot(wi + x * 16 + (lane / 16) * 4, wj + y * 16 + lane % 16)] = PARTS == 3 ? acc[x][y] + low[x][y] : acc[x][y];
     __syncthreads();
     float scale = p.scale;
     if (p.inv_power) scale *= p.inv_power == 1 ? p.inv[b] : p.inv[b] * p.inv[b];
@@ -394,7 +390,7 @@ __global__ __launch_bounds__(256, TILE <= 128 && STAGES * TILE <= 256 ? 2 : 1) v
     };
     if (WHAT == STEP || (WHAT == LAST && p.tall) || ((WHAT == SYM || WHAT == POLY) && ti != tj)) {
 #pragma unroll 2
-        for (int k = tid; k < TILE * TILE / 8; k += 256) {
+        for (int k = tid; k < TILE * TILE / 8; k += WAVES * WAVE) {
             const int j = k / (TILE / 8), i = k % (TILE / 8) * 8;
             float v[8];
             *(float4_*)v = *(const float4_*)&res[spot(i, j)], *(float4_*)(v + 4) = *(const float4_*)&res[spot(i, j) + 4];
@@ -403,7 +399,7 @@ __global__ __launch_bounds__(256, TILE <= 128 && STAGES * TILE <= 256 ? 2 : 1) v
     }
     if (WHAT != LAST || !p.tall) {
 #pragma unroll 2
-        for (int k = tid; k < TILE * TILE / 8; k += 256) {
+        for (int k = tid; k < TILE * TILE / 8; k += WAVES * WAVE) {
             const int g = k / WAVE, i = g % (TILE / 16) * 16 + lane % 16, j = g / (TILE / 16) * 32 + lane / 16 * 8;
             float v[8];
 #pragma unroll
@@ -479,11 +475,11 @@ static bool ranges(Plan* q) {
     return true;
 }
 
-template <class T, int WHAT, int PARTS, int TILE, int STAGES>
+template <class T, int WHAT, int PARTS, int TILE, int STAGES, int WAVES>
 static void launch_tiles(const Product& p, const Product* second, int batch, hipStream_t s) {
     const int rows = (p.rows + TILE - 1) / TILE, cols = (p.cols + TILE - 1) / TILE;
     const int tiles = WHAT == SYM || WHAT == POLY ? rows * (rows + 1) / 2 : rows * cols;
-    product_kernel<T, WHAT, PARTS, TILE, STAGES><<<dim3(tiles, 1, second ? 2 * batch : batch), 256, 0, s>>>(p, second ? *second : p, batch);
+    product_kernel<T, WHAT, PARTS, TILE, STAGES, WAVES><<<dim3(tiles, 1, second ? 2 * batch : batch), WAVES * WAVE, 0, s>>>(p, second ? *second : p, batch);
 }
 // The tile: the one with which the compute unit that has the most of them is done first.  What a tile takes, in us, measured with
 // three products a K-step at 4000 x 4100 (all units busy) and 128 x 256 (a few steps): 64: 0.31 a step and 1.5 beside, 128: 0.72 and 4,
@@ -498,13 +494,13 @@ static void launch_product(const Product& p, const Product* second, int batch, h
     };
     const double t64 = rounds(64) * (0.31 * steps + 1.5), t128 = rounds(128) * (0.72 * steps + 4), t192 = rounds(192) * (1.32 * steps + 8);
     if (t192 < t128 && t192 < t64)
-        launch_tiles<T, WHAT, PARTS, 192, 3>(p, second, batch, s);
+        launch_tiles<T, WHAT, PARTS, 192, 3, PARTS == 2 ? 4 : 8>(p, second, batch, s);
     else if (t128 < t64 && rounds(128) == 1)
-        launch_tiles<T, WHAT, PARTS, 128, 4>(p, second, batch, s);
+        launch_tiles<T, WHAT, PARTS, 128, 4, 4>(p, second, batch, s);
     else if (t128 < t64)
-        launch_tiles<T, WHAT, PARTS, 128, 2>(p, second, batch, s);
+        launch_tiles<T, WHAT, PARTS, 128, 2, 4>(p, second, batch, s);
     else
-        launch_tiles<T, WHAT, PARTS, 64, 4>(p, second, batch, s);
+        launch_tiles<T, WHAT, PARTS, 64, 4, 4>(p, second, batch, s);
 }
 
 static Product square(const Plan& q, Split l, Split r, Split o) {

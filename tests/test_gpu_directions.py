@@ -16,8 +16,8 @@ DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 ABC = directions.COEFFICIENTS
 
 
-def in_64_bits(g, steps, abc):
-    x = g.double().cpu()
+def in_64_bits(g, steps, abc, device="cpu"):
+    x = g.double().to(device)
     tall = x.shape[-2] > x.shape[-1]
     x = x.mT if tall else x
     n = x.square().sum((-2, -1), keepdim=True).sqrt()
@@ -54,6 +54,22 @@ def tolerance(g, trail, abc, dtype):
                 off += float(slope.abs().max()) * 3 * 2.0 ** -12 * scale * norms[j]
         worst = max(worst, off / norms[-1])
     return worst + torch.finfo(dtype).eps / 2
+
+
+def check_large(g, steps=5):
+    """The same in the Frobenius norm of the whole, with the 64-bit products on the GPU and the errors' growth from the power
+    iteration's bound on |X| (singular values of [0, 1.21] are within the polynomial's range): a^(steps left), at most."""
+    got = directions.orthogonalize(g, steps=steps).double()
+    flat = g.reshape(-1, *g.shape[-2:])
+    for k, x in enumerate(got.reshape(flat.shape)):
+        want, trail = in_64_bits(flat[k], steps, ABC, "cuda")
+        norms = [float(t.norm()) for t in trail]
+        off = sum(ABC[0] ** (steps - j) * 12 * 2.0 ** -23 * ABC[0] * norms[j] for j in range(steps + 1)) / norms[-1]
+        if g.dtype != torch.float32:
+            off = 1e-3  # the last steps on the Gram matrix
+        assert float((x - want).norm()) <= (off + torch.finfo(g.dtype).eps / 2) * norms[-1], (k, float((x - want).norm()) / norms[-1], off)
+        # and nowhere far off: no block of the result is another's
+        assert float((x - want).abs().max()) <= 40 * (off + torch.finfo(g.dtype).eps / 2) * max(norms[-1] / want.numel() ** 0.5, float(want.abs().max()) / 8)
 
 
 def check(g, steps=5, abc=ABC):
@@ -98,6 +114,13 @@ def test_batches(shape, dtype):
 @pytest.mark.parametrize("shape", [(700, 900), (1500, 500), (512, 2100), (1030, 1030)])
 def test_larger(shape, dtype):
     check(gradient(*shape, dtype=DT[dtype], rank=32))
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("shape", [(2100, 2300), (4000, 4100), (1100, 8200), (4, 1024, 2048), (3, 1500, 700), (12, 520, 600), (40, 260, 300)])
+def test_every_tile(shape, dtype):
+    """Sizes at which products go by tiles of 64, 128 (one and two to a unit) and 192, single and paired."""
+    check_large(gradient(*shape, dtype=DT[dtype], rank=64))
 
 
 @pytest.mark.parametrize("dtype", DT)
