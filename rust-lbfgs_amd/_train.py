@@ -6,7 +6,6 @@ operators do.  There is no CPU fallback: without the built library, or with tens
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import os
 
@@ -90,25 +89,24 @@ def floating(name, t):
         raise TypeError(f"{name} must be float64, float32, bfloat16 or float16, not {t.dtype}")
 
 
-def on_gpu(first, **others):
-    """The one device of these tensors (None: absent)."""
-    name, t = first
-    if t.device.type != "cuda":
-        raise TypeError(f"{name} is on {t.device}: the operators run on the GPU, there is no CPU fallback")
-    for other, o in others.items():
-        if o is not None and o.device != t.device:
-            raise ValueError(f"{other} is on {o.device}, {name} on {t.device}")
-    return t.device
+def on_gpu(name, t, others=()):
+    """The one device of these tensors, (name, tensor or None) each."""
+    dev = t.device
+    if dev.type != "cuda":
+        raise TypeError(f"{name} is on {dev}: the operators run on the GPU, there is no CPU fallback")
+    for other, o in others:
+        if o is not None and o.device != dev:
+            raise ValueError(f"{other} is on {o.device}, {name} on {dev}")
+    return dev
 
 
-def like(name, t, what, of, dtype=None, shape=None):
-    """`t` has the element type and shape of `of` (or the given ones)."""
+def like(name, t, what, dtype, shape):
+    """`t` has this element type and shape."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch tensor, not {type(t).__name__}")
-    dtype, shape = dtype or of.dtype, of.shape if shape is None else shape
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype} as {what} asks for, not {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)} as {what} asks for, not {tuple(t.shape)}")
 
 
@@ -116,13 +114,15 @@ def ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def stream_of(device):
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-def current(device):
-    """The kernels are enqueued with the tensors' device as the current one."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def enqueue(function, device, *arguments):
+    """`function(*arguments, stream)` with the tensors' device as the current one, on its current stream."""
+    if torch.cuda.current_device() == device.index:
+        rc = function(*arguments, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device):
+            rc = function(*arguments, torch._C._cuda_getCurrentRawStream(device.index))
+    if rc != 0:
+        check(rc)
 
 
 def refuse_capture(what, instead):

@@ -23,9 +23,13 @@ __device__ __forceinline__ double lowest<double>() {
     return -1.7976931348623157e+308;
 }
 
+// (the larger of two, of three in one instruction; a NaN is passed over here and shows in the sum)
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_fmaxf(a, b); }
+__device__ __forceinline__ double larger(double a, double b) { return __builtin_fmax(a, b); }
+
 template <class A>
 __device__ __forceinline__ void join(MaxSum<A>& a, A m, A s, A c) {
-    const A M = m > a.m ? m : a.m;
+    const A M = larger(a.m, m);
     a.s = a.s * exp2_of((a.m - M) * c) + s * exp2_of((m - M) * c);
     a.m = M;
 }
@@ -34,14 +38,11 @@ __device__ __forceinline__ void join(MaxSum<A>& a, A m, A s, A c) {
 // (x - m is exact for 16-bit logits), so the scale's own rounding stays a relative error of the exponent's size.
 template <class T, int N, int U, class A>
 __device__ __forceinline__ void add(MaxSum<A>& a, const Pack<T, N> (&p)[U], A c) {
-    A v = (A)p[0].v[0];
+    A v = a.m;
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
-        for (int k = 0; k < N; k++) {
-            const A x = (A)p[u].v[k];
-            v = x > v ? x : v;
-        }
+        for (int k = 0; k < N; k++) v = larger(v, (A)p[u].v[k]);
     if (v > a.m) {
         a.s *= exp2_of((a.m - v) * c);
         a.m = v;
@@ -106,11 +107,17 @@ __device__ __forceinline__ const T* row_at(const T* x, const Rows& r, int64_t ro
     return x + (row / r.inner) * r.outer_stride + (row % r.inner) * r.inner_stride;
 }
 
-template <class T, class A>
-__device__ __forceinline__ void finish_row(const T* x, const Rows& r, int64_t y, MaxSum<A> a, double tau, A* logp, double* lse) {
+// the target's logit, asked for before the row is read (NaN: there is none)
+template <class T>
+__device__ __forceinline__ typename Num<T>::acc target(const T* x, const Rows& r, int64_t y) {
+    typedef typename Num<T>::acc A;
+    return y >= 0 && y < r.vocab ? (A)x[y] : (A)NAN;
+}
+template <class A>
+__device__ __forceinline__ void finish_row(A chosen, MaxSum<A> a, double tau, A* logp, double* lse) {
     // (x_y - m) - log s: nothing as large as the logits themselves is rounded, and a row masked by the type's lowest value
     // throughout keeps its log s
-    *logp = y >= 0 && y < r.vocab ? (A)(((double)(A)x[y] - (double)a.m) / tau) - log(a.s) : (A)NAN;
+    *logp = (A)(((double)chosen - (double)a.m) / tau) - log(a.s);
     lse[0] = (double)a.m;
     lse[1] = log((double)a.s);
 }
@@ -124,8 +131,9 @@ __global__ __launch_bounds__(BLOCK) void logprobs_kernel(const T* x, Rows r, dou
             continue;
         }
         const T* at = row_at(x, r, row);
+        const auto chosen = target(at, r, y);
         const auto a = row_part<T, BLOCK>(at, r.vocab, c);
-        if (threadIdx.x == 0) finish_row(at, r, y, a, tau, logps + row, lse + 2 * row);
+        if (threadIdx.x == 0) finish_row(chosen, a, tau, logps + row, lse + 2 * row);
         __syncthreads();  // row_part's shared memory is written again
     }
 }
@@ -147,25 +155,25 @@ __global__ __launch_bounds__(WAVE) void logprobs_join_kernel(const T* x, Rows r,
         if (threadIdx.x == 0) logps[row] = 0, lse[2 * row] = 0, lse[2 * row + 1] = 0;
         return;
     }
+    const A chosen = target(row_at(x, r, row), r, y);
     MaxSum<A> a = {lowest<A>(), (A)0};
     for (int k = threadIdx.x; k < splits; k += WAVE) join(a, found[row * splits + k].m, found[row * splits + k].s, c);
 #pragma unroll
     for (int o = WAVE / 2; o; o >>= 1) join(a, shfl_xor(a.m, o), shfl_xor(a.s, o), c);
-    if (threadIdx.x == 0) finish_row(row_at(x, r, row), r, y, a, tau, logps + row, lse + 2 * row);
+    if (threadIdx.x == 0) finish_row(chosen, a, tau, logps + row, lse + 2 * row);
 }
 
 // The gradient: element-wise once the row's maximum and sum are known, so a row is cut into as many parts as fill the chip.
 template <class T, int N, class A>
-__device__ __forceinline__ void grad_pack(const T* x, T* dx, int64_t v, int64_t y, A hi, A c, A scale, A at_target) {
-    const Pack<T, N> p = *(const Pack<T, N>*)(x + v);
+__device__ __forceinline__ void grad_pack(const Pack<T, N>& p, T* dx, int64_t v, int64_t y, A hi, A c, A scale, A at_target) {
     Pack<T, N> d;
+#pragma unroll
+    for (int k = 0; k < N; k++) d.v[k] = (T)(scale * exp2_of(((A)p.v[k] - hi) * c));
     const uint64_t off = (uint64_t)(y - v);
     if (off < (uint64_t)N) {
 #pragma unroll
-        for (int k = 0; k < N; k++) d.v[k] = (T)((uint64_t)k == off ? at_target : scale * exp2_of(((A)p.v[k] - hi) * c));
-    } else {
-#pragma unroll
-        for (int k = 0; k < N; k++) d.v[k] = (T)(scale * exp2_of(((A)p.v[k] - hi) * c));
+        for (int k = 0; k < N; k++)
+            if ((uint64_t)k == off) d.v[k] = (T)at_target;
     }
     if (N == 1)
         dx[v] = d.v[0];
@@ -180,7 +188,8 @@ __global__ __launch_bounds__(BLOCK) void logprobs_grad_kernel(const T* x, Rows r
     constexpr int N = vec_len<T>(), U = 4;
     const int tid = threadIdx.x;
     for (int64_t unit = blockIdx.x; unit < r.rows * splits; unit += gridDim.x) {
-        const int64_t row = unit / splits, lo = (unit % splits) * part, hi_v = lo + part < r.vocab ? lo + part : r.vocab;
+        // the last rows first: what the forward pass read last is in the caches yet
+        const int64_t row = r.rows - 1 - unit / splits, lo = (unit % splits) * part, hi_v = lo + part < r.vocab ? lo + part : r.vocab;
         const int64_t y = r.targets[row];
         const A g = y == r.ignore ? (A)0 : grad[row];
         T* out = dx + row * r.vocab;
@@ -207,12 +216,16 @@ __global__ __launch_bounds__(BLOCK) void logprobs_grad_kernel(const T* x, Rows r
         A at_target = 0;
         if (y >= lo && y < hi_v) at_target = -coef * (A)expm1(((double)(A)in[y] - (double)hi) / tau - l);
         int64_t i = tid;
-        for (; i + (U - 1) * BLOCK < packs; i += U * BLOCK)
+        for (; i + (U - 1) * BLOCK < packs; i += U * BLOCK) {
+            Pack<T, N> p[U];
 #pragma unroll
-            for (int u = 0; u < U; u++) grad_pack<T, N, A>(in, out, head + (i + u * BLOCK) * N, y, hi, c, scale, at_target);
-        for (; i < packs; i += BLOCK) grad_pack<T, N, A>(in, out, head + i * N, y, hi, c, scale, at_target);
-        for (int64_t k = lo + tid; k < head; k += BLOCK) grad_pack<T, 1, A>(in, out, k, y, hi, c, scale, at_target);
-        for (int64_t k = done + tid; k < hi_v; k += BLOCK) grad_pack<T, 1, A>(in, out, k, y, hi, c, scale, at_target);
+            for (int u = 0; u < U; u++) p[u] = *(const Pack<T, N>*)(in + head + (i + u * BLOCK) * N);
+#pragma unroll
+            for (int u = 0; u < U; u++) grad_pack<T, N, A>(p[u], out, head + (i + u * BLOCK) * N, y, hi, c, scale, at_target);
+        }
+        for (; i < packs; i += BLOCK) grad_pack<T, N, A>(*(const Pack<T, N>*)(in + head + i * N), out, head + i * N, y, hi, c, scale, at_target);
+        for (int64_t k = lo + tid; k < head; k += BLOCK) grad_pack<T, 1, A>({{in[k]}}, out, k, y, hi, c, scale, at_target);
+        for (int64_t k = done + tid; k < hi_v; k += BLOCK) grad_pack<T, 1, A>({{in[k]}}, out, k, y, hi, c, scale, at_target);
     }
 }
 
@@ -248,10 +261,10 @@ static void launch_forward(const void* x, const Rows& r, double tau, void* logps
         logprobs_join_kernel<T><<<(unsigned)r.rows, WAVE, 0, s>>>((const T*)x, r, tau, c, splits, found, (A*)logps, lse);
     } else if (bytes <= 4096) {
         logprobs_kernel<T, 64><<<(unsigned)grid, 64, 0, s>>>((const T*)x, r, tau, c, (A*)logps, lse);
-    } else if (bytes <= 65536 || r.rows >= 2048) {
+    } else if (bytes <= 131072) {  // (a row of 64 KiB: 112 us for 8192 of them with 128, 256 or 512 threads, 148 with 1024)
         logprobs_kernel<T, 256><<<(unsigned)grid, 256, 0, s>>>((const T*)x, r, tau, c, (A*)logps, lse);
-    } else {
-        logprobs_kernel<T, 1024><<<(unsigned)grid, 1024, 0, s>>>((const T*)x, r, tau, c, (A*)logps, lse);
+    } else {  // (256 KiB: 351 us with 256, 346 with 512, 354 with 1024)
+        logprobs_kernel<T, 512><<<(unsigned)grid, 512, 0, s>>>((const T*)x, r, tau, c, (A*)logps, lse);
     }
 }
 

@@ -15,12 +15,20 @@ namespace lt {
 constexpr int E = 8;             // adjacent tokens of a thread: one 16-byte load of 16-bit values, two of 32
 constexpr int BLOCK = 256, CHUNK = BLOCK * E;
 constexpr int LOSS_BLOCKS = 1024;   // workgroups of the pass over pairs, each leaving one partial loss
-constexpr int COUNT_BLOCKS = 64;    // ... of the pass over sequences of the policy loss
+constexpr int COUNT_BLOCKS = 256;   // ... of the pass of the policy loss that counts
 constexpr int POLICY_BLOCKS = 2048; // ... of its pass over tokens
+constexpr int FAR = 1 << 30;        // a distance in tokens beyond every chunk
 
 struct Rec {
     double sum;
     int64_t count;
+};
+
+// Where a thread is in the sequences: number s, and the distances of its first and behind its last token from the thread's own
+// first one (FAR where there is none; a sequence that started long ago: some negative number)
+struct Spot {
+    int64_t s;
+    int begin, end;
 };
 
 // the sequences: offsets [seqs + 1] in 32 or 64 bits, or `longest` tokens each.  Offsets are data of the device that the
@@ -39,20 +47,108 @@ struct Seqs {
         return o < 0 ? 0 : o > tokens ? tokens : o;
     }
     __device__ __forceinline__ bool good(int64_t s) const { return raw(s) >= 0 && raw(s) <= raw(s + 1) && raw(s + 1) <= tokens; }
-    // the sequence of token t: the last that starts at or before it; `count` where there is none
-    __device__ __forceinline__ int64_t of(int64_t t) const {
-        if (t >= tokens) return count;
-        if (bits == 0) return t / longest;
-        int64_t lo = -1, hi = count;  // at(lo) <= t < at(hi), taking at(-1) = -inf
+    __device__ __forceinline__ static int distance(int64_t d) { return d > FAR ? FAR : d < -FAR ? -FAR : (int)d; }
+
+    // The sequence of the thread's first token t (of its wave's: t - lane * E): the last that starts at or before it.  A whole
+    // wave looks for its first token's, 64 offsets a round, and then has the next 64 offsets in its lanes: one to three rounds
+    // of loads that wait for each other where a search of each thread's own had twelve.
+    __device__ __forceinline__ Spot locate(int64_t t) const {
+        if (bits == 0) {
+            if (t >= tokens) return {count, FAR, FAR};
+            const int64_t s = tokens < (int64_t)1 << 32 ? (int64_t)((uint32_t)t / (uint32_t)longest) : t / longest;
+            return {s, distance(s * longest - t), distance((s + 1) * longest - t)};
+        }
+        const int lane = threadIdx.x % WAVE;
+        const int64_t first = t - lane * E;
+        int64_t lo = -1, hi = count;  // at(lo) <= first < at(hi), at(-1) being -inf
+        while (hi - lo > WAVE) {
+            const int64_t step = (hi - lo + WAVE - 1) / WAVE, probe = lo + step * (lane + 1);
+            const int n = __popcll(__ballot(probe < hi && at(probe) <= first));
+            lo += step * n;
+            if (lo + step < hi) hi = lo + step;
+        }
+        const int64_t here = lo + 1 + lane;
+        const int64_t value = here <= count ? at(here) : INT64_MAX;
+        const int past = __popcll(__ballot(here < hi && value <= first));
+        // the offsets that follow the first token, from these as far as they reach
+        const int known = value == INT64_MAX ? FAR : distance(value - first);
+        int next = __shfl(known, (lane + past) % WAVE, WAVE);
+        int start = __shfl(known, past ? past - 1 : 0, WAVE);
+        if (past == 0) start = lo >= 0 ? distance(at(lo) - first) : 0;
+        lo += past;
+        if (lane + past >= WAVE) next = lo + 1 + lane <= count ? distance(at(lo + 1 + lane) - first) : FAR;
+        const int own = lane * E;
+        int n = 0;  // how many of them are at or before t
+#pragma unroll
+        for (int o = WAVE / 2; o; o >>= 1)
+            if (__shfl(next, n + o - 1, WAVE) <= own) n += o;
+        const bool beyond = n == WAVE - 1 && __shfl(next, WAVE - 1, WAVE) <= own;
+        const int before = __shfl(next, n ? n - 1 : 0, WAVE), after = __shfl(next, n, WAVE), second = __shfl(next, 1, WAVE);
+        int64_t s = lo + n;
+        int begin = n ? before : start, end = after;
+        if (beyond) {  // more than 64 sequences begin among the tokens of a wave: a search of the thread's own
+            int64_t h = count;
+            s = lo + WAVE;
+            while (h - s > 1) {
+                const int64_t mid = (s + h) >> 1;
+                if (at(mid) <= t)
+                    s = mid;
+                else
+                    h = mid;
+            }
+            begin = distance(at(s) - first), end = s < count ? distance(at(s + 1) - first) : FAR;
+        }
+        if (s < 0) s = 0, begin = after, end = second;  // before the first sequence
+        if (s >= count || (end != FAR && end <= own)) return {count, FAR, FAR};
+        return {s, begin - own, end == FAR ? FAR : end - own};
+    }
+    // behind sequence at.s, which ends at `t + at.end`: the next one that has tokens
+    __device__ __forceinline__ void next(Spot& at_, int64_t t) const {
+        const int64_t from = t + at_.end;
+        int64_t s = at_.s;
+        do {
+            s++;
+        } while (s < count && at(s + 1) <= from);
+        at_ = s < count ? Spot{s, distance(at(s) - t), distance(at(s + 1) - t)} : Spot{count, FAR, FAR};
+    }
+};
+
+// The same of a small batch, its offsets in LDS
+constexpr int SMALL_CHUNKS = 2, SMALL_TOKENS = SMALL_CHUNKS * CHUNK, SMALL_SEQS = 256;
+struct SmallSeqs {
+    const int* offsets;          // clamped
+    const uint8_t* fine;         // good()
+    int64_t tokens, count;
+    const uint8_t* mask;
+    __device__ __forceinline__ int64_t at(int64_t s) const { return offsets[s]; }
+    __device__ __forceinline__ bool good(int64_t s) const { return fine[s]; }
+    __device__ __forceinline__ Spot locate(int64_t t) const {
+        int lo = -1, hi = (int)count;
         while (hi - lo > 1) {
-            const int64_t mid = (lo + hi) >> 1;
-            if (at(mid) <= t)
+            const int mid = (lo + hi) >> 1;
+            if (offsets[mid] <= t)
                 lo = mid;
             else
                 hi = mid;
         }
-        return lo < 0 ? 0 : lo;
+        if (lo < 0) lo = 0;
+        if (offsets[lo + 1] <= t) return {count, FAR, FAR};
+        return {lo, offsets[lo] - (int)t, offsets[lo + 1] - (int)t};
     }
+    __device__ __forceinline__ void next(Spot& at_, int64_t t) const {
+        const int from = (int)t + at_.end;
+        int s = (int)at_.s;
+        do {
+            s++;
+        } while (s < count && offsets[s + 1] <= from);
+        at_ = s < count ? Spot{s, offsets[s] - (int)t, offsets[s + 1] - (int)t} : Spot{count, FAR, FAR};
+    }
+};
+struct SmallSpace {
+    int offsets[SMALL_SEQS + 1];
+    uint8_t fine[SMALL_SEQS];
+    Rec total[SMALL_SEQS], head[SMALL_CHUNKS], tail[SMALL_CHUNKS];
+    double slope[SMALL_SEQS], loss[1], counts[2];
 };
 
 struct Space {  // the workspace
@@ -63,26 +159,14 @@ struct Space {  // the workspace
     double* sums;        // [POLICY_BLOCKS][3]: loss, KL, clipped
 };
 
-// A thread's place in the sequences as it walks its tokens
-struct Walk {
-    int64_t s, begin, end;
-    __device__ __forceinline__ void start(const Seqs& q, int64_t t) {
-        s = q.of(t);
-        begin = s < q.count ? q.at(s) : INT64_MAX;
-        end = s < q.count ? q.at(s + 1) : INT64_MAX;
-        if (end <= t && s < q.count) s = q.count, begin = end = INT64_MAX;  // behind the last sequence
+__device__ __forceinline__ SmallSeqs small_seqs(const Seqs& q, SmallSpace& m, Space& sp) {
+    for (int s = threadIdx.x; s <= q.count; s += BLOCK) {
+        m.offsets[s] = (int)q.at(s);
+        if (s < q.count) m.fine[s] = q.good(s);
     }
-    __device__ __forceinline__ bool inside(int64_t t) const { return t >= begin; }
-    // past the end of sequence s: the next one that has tokens
-    __device__ __forceinline__ void next(const Seqs& q) {
-        const int64_t t = end;
-        do {
-            s++;
-        } while (s < q.count && q.at(s + 1) <= t);
-        begin = s < q.count ? q.at(s) : INT64_MAX;
-        end = s < q.count ? q.at(s + 1) : INT64_MAX;
-    }
-};
+    sp.total = m.total, sp.head = m.head, sp.tail = m.tail, sp.slope = m.slope, sp.loss = m.loss, sp.counts = m.counts;
+    return {m.offsets, m.fine, q.tokens, q.count, q.mask};
+}
 
 template <class T>
 __device__ __forceinline__ void load(const T* p, int64_t t, int64_t n, Pack<T, E>& out) {
@@ -101,49 +185,52 @@ __device__ __forceinline__ void store(T* p, int64_t t, int64_t n, const Pack<T, 
         for (int k = 0; k < E; k++)
             if (t + k < n) p[t + k] = in.v[k];
 }
-__device__ __forceinline__ void load_mask(const Seqs& q, int64_t t, Pack<uint8_t, E>& keep) {
-    if (q.mask) {
-        load(q.mask, t, q.tokens, keep);
+__device__ __forceinline__ void load_mask(const uint8_t* mask, int64_t t, int64_t n, Pack<uint8_t, E>& keep) {
+    if (mask) {
+        load(mask, t, n, keep);
     } else {
 #pragma unroll
         for (int k = 0; k < E; k++) keep.v[k] = 1;
     }
 }
 
-// Sums of (a - b) and counts over the sequences of chunk w (a NULL: counts alone; b NULL: 0).  A thread adds up its own
-// tokens; a scan over the threads that restarts wherever a sequence ends carries the rest.
+// a thread's tokens of two tensors (a NULL: none are wanted; b NULL: zeros)
 template <class T>
-__device__ __forceinline__ void chunk_sums(const Seqs& q, const T* a, const T* b, int64_t w, const Space& sp) {
+struct Tokens {
+    Pack<T, E> a, b;
+    Pack<uint8_t, E> keep;
+    __device__ __forceinline__ void get(const uint8_t* mask, const T* pa, const T* pb, int64_t t, int64_t n) {
+        load_mask(mask, t, n, keep);
+        if (pa) load(pa, t, n, a);
+        if (pb) load(pb, t, n, b);
+    }
+};
+
+// Sums of (a - b) and counts over the sequences of chunk w.  A thread adds up its own tokens; a scan over the threads that restarts
+// wherever a sequence ends carries the rest.
+template <class T, class Q>
+__device__ __forceinline__ void chunk_sums(const Q& q, const Tokens<T>& x, bool has_a, bool has_b, int64_t w, const Space& sp) {
     __shared__ double wave_sum_[BLOCK / WAVE];
     __shared__ int wave_count_[BLOCK / WAVE], wave_closed_[BLOCK / WAVE];
     const int tid = threadIdx.x, lane = tid % WAVE, wave = tid / WAVE;
-    const int64_t chunk = w * CHUNK, t0 = chunk + tid * E;
-    Walk at;
-    at.start(q, t0);
-    Pack<T, E> x, y;
-    Pack<uint8_t, E> keep;
-    load_mask(q, t0, keep);
-    if (a) load(a, t0, q.tokens, x);
-    if (b) load(b, t0, q.tokens, y);
+    const int64_t t0 = w * CHUNK + tid * E;
+    Spot at = q.locate(t0);
     double sum = 0, first_sum = 0;
-    int count = 0, first_count = 0;
-    int64_t first = -1, first_begin = 0;  // the first sequence that ends among this thread's tokens
+    int count = 0, first_count = 0, first_begin = 0;
+    int64_t first = -1;  // the first sequence that ends among this thread's tokens
 #pragma unroll
     for (int k = 0; k < E; k++) {
-        const int64_t t = t0 + k;
-        if (t < q.tokens) {
-            if (at.inside(t) && keep.v[k]) {  // (what is masked is not looked at: it may be anything)
-                if (a) sum += b ? (double)x.v[k] - (double)y.v[k] : (double)x.v[k];
-                count++;
-            }
-            if (t + 1 == at.end) {
-                if (first < 0)
-                    first = at.s, first_begin = at.begin, first_sum = sum, first_count = count;
-                else
-                    sp.total[at.s] = {sum, count};
-                sum = 0, count = 0;
-                at.next(q);
-            }
+        if (k >= at.begin && k < at.end && x.keep.v[k]) {  // (what is masked is not looked at: it may be anything)
+            if (has_a) sum += has_b ? (double)x.a.v[k] - (double)x.b.v[k] : (double)x.a.v[k];
+            count++;
+        }
+        if (k + 1 == at.end) {
+            if (first < 0)
+                first = at.s, first_begin = at.begin, first_sum = sum, first_count = count;
+            else
+                sp.total[at.s] = {sum, count};
+            sum = 0, count = 0;
+            q.next(at, t0);
         }
     }
     // inclusive scan of (closed, sum, count): (c1, v1) + (c2, v2) = (c1 | c2, c2 ? v2 : v1 + v2)
@@ -173,15 +260,15 @@ __device__ __forceinline__ void chunk_sums(const Seqs& q, const T* a, const T* b
     if (!in_closed) in += before, in_count += before_count;
     if (first >= 0) {
         const Rec r = {in + first_sum, in_count + first_count};
-        if (first_begin >= chunk)
+        if (first_begin + tid * E >= 0)  // it began in this chunk
             sp.total[first] = r;
         else
             sp.head[w] = r;
     }
-    if (tid == BLOCK - 1 && at.s < q.count && at.begin < chunk + CHUNK) {  // goes on behind the chunk
+    if (tid == BLOCK - 1 && at.s < q.count && at.begin < E) {  // goes on behind the chunk
         Rec r = {sum, count};
         if (first < 0) r.sum += in, r.count += in_count;
-        if (at.begin >= chunk)
+        if (at.begin + tid * E >= 0)
             sp.tail[w] = r;
         else
             sp.head[w] = r;
@@ -190,8 +277,8 @@ __device__ __forceinline__ void chunk_sums(const Seqs& q, const T* a, const T* b
 }
 
 // the whole of sequence s, by GROUP adjacent lanes; every one of them gets it
-template <int GROUP>
-__device__ __forceinline__ Rec sequence(const Seqs& q, const Space& sp, int64_t s, int l) {
+template <int GROUP, class Q>
+__device__ __forceinline__ Rec sequence(const Q& q, const Space& sp, int64_t s, int l) {
     const int64_t begin = q.at(s), end = q.at(s + 1);
     Rec r = {0, 0};
     if (end > begin) {
@@ -200,7 +287,15 @@ __device__ __forceinline__ Rec sequence(const Seqs& q, const Space& sp, int64_t 
             if (l == 0) r = sp.total[s];
         } else {
             if (l == 0) r = sp.tail[w0];
-            for (int64_t w = w0 + 1 + l; w <= w1; w += GROUP) r.sum += sp.head[w].sum, r.count += sp.head[w].count;
+            int64_t w = w0 + 1 + l;
+            for (; w + 3 * GROUP <= w1; w += 4 * GROUP) {  // (four loads under way at once)
+                Rec v[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[k] = sp.head[w + k * GROUP];
+#pragma unroll
+                for (int k = 0; k < 4; k++) r.sum += v[k].sum, r.count += v[k].count;
+            }
+            for (; w <= w1; w += GROUP) r.sum += sp.head[w].sum, r.count += sp.head[w].count;
         }
     }
 #pragma unroll
@@ -208,7 +303,7 @@ __device__ __forceinline__ Rec sequence(const Seqs& q, const Space& sp, int64_t 
     return r;
 }
 
-__device__ __forceinline__ double block_sum(double v) {  // valid in thread 0
+__device__ __forceinline__ double block_sum(double v) {
     __shared__ double part[BLOCK / WAVE];
     v = wave_sum(v);
     if (threadIdx.x % WAVE == 0) part[threadIdx.x / WAVE] = v;
@@ -224,69 +319,73 @@ struct Preference {
     double beta, smoothing;
     int kind, normalize;
 };
+struct Pair {
+    double loss, preferred, rejected;  // d loss / d token of its sequences, of the mean over the pairs
+    double d_preferred, d_rejected;    // their R
+};
 
 // Pair i compares sequence i with sequence i + pairs.  In terms of the difference D of the two sums, h = beta D:
 //   logistic  -(1-e) log sig(h) - e log sig(-h)      d/dD = beta (e - sig(-h))
 //   hinge     max(0, 1 - h)                          d/dD = -beta where h < 1
 //   squared   (D - 1/(2 beta))^2                     d/dD = 2 (D - 1/(2 beta))
-template <class A>
-__device__ __forceinline__ void pair_losses(const Seqs& q, const Preference& o, const Space& sp, A* rewards, int block, int blocks) {
-    constexpr int GROUP = 8;
-    const int64_t pairs = q.count / 2;
+__device__ __forceinline__ Pair pair_of(const Preference& o, const Rec& c, const Rec& r, bool good, int64_t pairs) {
+    const double nc = o.normalize && c.count ? 1.0 / (double)c.count : 1.0, nr = o.normalize && r.count ? 1.0 / (double)r.count : 1.0;
+    const double dc = c.sum * nc, dr = r.sum * nr, D = good ? dc - dr : NAN, h = o.beta * D;
+    double loss, slope;
+    if (o.kind == LBFGS_TRAIN_LOGISTIC) {
+        const double e = exp(-fabs(h)), soft = log1p(e);
+        loss = (1 - o.smoothing) * (soft + (h < 0 ? -h : 0)) + (o.smoothing != 0 ? o.smoothing * (soft + (h > 0 ? h : 0)) : 0);
+        if (h != h) loss = h;
+        slope = o.beta * (o.smoothing - (h < 0 ? 1.0 : e) / (1.0 + e));  // sig(-h)
+    } else if (o.kind == LBFGS_TRAIN_HINGE) {
+        loss = h > 1 ? 0 : 1 - h;
+        slope = h < 1 ? -o.beta : h != h ? h : 0;
+    } else {
+        const double e = D - 0.5 / o.beta;
+        loss = e * e;
+        slope = 2 * e;
+    }
+    slope /= (double)pairs;
+    return {loss, slope * nc, -slope * nr, dc, dr};
+}
+
+// pairs [block], [block + blocks], ... in groups: losses into sp.loss[block], rewards, and -- if they are asked for -- slopes
+template <int GROUP, class A, class Q>
+__device__ __forceinline__ void pair_losses(const Q& q, const Preference& o, const Space& sp, A* rewards, bool slopes, int block, int blocks) {
+    const int64_t pairs = q.count / 2, each = (int64_t)blocks * (BLOCK / GROUP), rounds = (pairs + each - 1) / each;
     const int l = threadIdx.x % GROUP;
-    const int64_t rounds = (pairs + (int64_t)blocks * (BLOCK / GROUP) - 1) / ((int64_t)blocks * (BLOCK / GROUP));
     double total = 0;
     for (int64_t k = 0; k < rounds; k++) {  // (every lane goes through the shuffles of sequence())
-        const int64_t i = (k * blocks + block) * (BLOCK / GROUP) + threadIdx.x / GROUP;
+        const int64_t i = k * each + (int64_t)block * (BLOCK / GROUP) + threadIdx.x / GROUP;
         const bool real = i < pairs;
         const Rec c = sequence<GROUP>(q, sp, real ? i : 0, l), r = sequence<GROUP>(q, sp, real ? i + pairs : 0, l);
         if (real && l == 0) {
-            const double nc = o.normalize && c.count ? 1.0 / (double)c.count : 1.0, nr = o.normalize && r.count ? 1.0 / (double)r.count : 1.0;
-            const double dc = c.sum * nc, dr = r.sum * nr, D = q.good(i) && q.good(i + pairs) ? dc - dr : NAN, h = o.beta * D;
-            double loss, slope;
-            if (o.kind == LBFGS_TRAIN_LOGISTIC) {
-                const double soft = log1p(exp(-fabs(h)));
-                loss = (1 - o.smoothing) * (soft + (h < 0 ? -h : 0)) + (o.smoothing != 0 ? o.smoothing * (soft + (h > 0 ? h : 0)) : 0);
-                if (h != h) loss = h;
-                slope = o.beta * (o.smoothing - 1.0 / (1.0 + exp(h)));
-            } else if (o.kind == LBFGS_TRAIN_HINGE) {
-                loss = h > 1 ? 0 : 1 - h;
-                slope = h < 1 ? -o.beta : h != h ? h : 0;
-            } else {
-                const double e = D - 0.5 / o.beta;
-                loss = e * e;
-                slope = 2 * e;
-            }
-            total += loss;
-            slope /= (double)pairs;
-            sp.slope[i] = slope * nc;
-            sp.slope[i + pairs] = -slope * nr;
-            rewards[i] = (A)(o.beta * dc);
-            rewards[i + pairs] = (A)(o.beta * dr);
+            const Pair p = pair_of(o, c, r, q.good(i) && q.good(i + pairs), pairs);
+            total += p.loss;
+            if (slopes) sp.slope[i] = p.preferred, sp.slope[i + pairs] = p.rejected;
+            rewards[i] = (A)(o.beta * p.d_preferred);
+            rewards[i + pairs] = (A)(o.beta * p.d_rejected);
         }
     }
     total = block_sum(total);
     if (threadIdx.x == 0) sp.loss[block] = total;
 }
 
-// gradient of chunk w: its sequence's slope at each token that counts, 0 at all others
-template <class T>
-__device__ __forceinline__ void chunk_slopes(const Seqs& q, const Space& sp, T* grad, int64_t w) {
+// gradient of chunk w: its sequence's slope at each token that counts, 0 at all others.  slope[(s - base) & within]: with a table of
+// the chunk's own sequences, bad offsets still lead nowhere else.
+template <class T, class Q>
+__device__ __forceinline__ void chunk_slopes(const Q& q, const double* slope, int64_t base, int64_t within, T* grad, int64_t w, Spot at, const Pack<uint8_t, E>& keep) {
+    typedef typename Num<T>::acc A;
     const int64_t t0 = w * CHUNK + threadIdx.x * E;
     if (t0 >= q.tokens) return;
-    Walk at;
-    at.start(q, t0);
-    Pack<uint8_t, E> keep;
-    load_mask(q, t0, keep);
     Pack<T, E> g;
-    typename Num<T>::acc slope = at.s < q.count ? (typename Num<T>::acc)sp.slope[at.s] : 0;
+    A v = at.s < q.count ? (A)slope[(at.s - base) & within] : 0;
 #pragma unroll
     for (int k = 0; k < E; k++) {
-        const int64_t t = t0 + k;
-        g.v[k] = at.inside(t) && keep.v[k] ? (T)slope : (T)0;
-        if (t + 1 == at.end) {
-            at.next(q);
-            if (k + 1 < E) slope = at.s < q.count ? (typename Num<T>::acc)sp.slope[at.s] : 0;
+        g.v[k] = k >= at.begin && k < at.end && keep.v[k] ? (T)v : (T)0;
+        if (k + 1 == at.end) {
+            q.next(at, t0);
+            if (k + 1 < E) v = at.s < q.count ? (A)slope[(at.s - base) & within] : 0;
         }
     }
     store(grad, t0, q.tokens, g);
@@ -301,28 +400,96 @@ __device__ __forceinline__ void mean_loss(const Space& sp, int blocks, int64_t p
 }
 
 template <class T>
-__global__ __launch_bounds__(BLOCK) void sums_kernel(Seqs q, const T* a, const T* b, int64_t chunks, Space sp) {
-    for (int64_t w = blockIdx.x; w < chunks; w += gridDim.x) chunk_sums(q, a, b, w, sp);
+__global__ __launch_bounds__(BLOCK, sizeof(T) == 8 ? 4 : 6) void sums_kernel(Seqs q, const T* a, const T* b, int64_t chunks, Space sp) {
+    for (int64_t w = blockIdx.x; w < chunks; w += gridDim.x) {
+        Tokens<T> x;
+        x.get(q.mask, a, b, w * CHUNK + threadIdx.x * E, q.tokens);
+        chunk_sums(q, x, a != nullptr, b != nullptr, w, sp);
+    }
 }
-template <class A>
+template <int GROUP, class A>
 __global__ __launch_bounds__(BLOCK) void pairs_kernel(Seqs q, Preference o, Space sp, A* rewards) {
-    pair_losses(q, o, sp, rewards, blockIdx.x, gridDim.x);
+    pair_losses<GROUP>(q, o, sp, rewards, true, blockIdx.x, gridDim.x);
 }
 template <class T>
 __global__ __launch_bounds__(BLOCK) void slopes_kernel(Seqs q, int64_t chunks, int blocks, Space sp, typename Num<T>::acc* f, T* grad) {
     if (blockIdx.x == 0) mean_loss(sp, blocks, q.count / 2, f);
-    for (int64_t w = blockIdx.x; w < chunks; w += gridDim.x) chunk_slopes(q, sp, grad, w);
+    for (int64_t w = blockIdx.x; w < chunks; w += gridDim.x) {
+        const int64_t t0 = w * CHUNK + threadIdx.x * E;
+        Pack<uint8_t, E> keep;
+        load_mask(q.mask, t0, q.tokens, keep);
+        chunk_slopes(q, sp.slope, 0, -1, grad, w, q.locate(t0), keep);
+    }
 }
-// a small batch: the three passes as one workgroup, so that one launch is all that is waited for
+// Not too many pairs: no pass of their own.  A chunk's workgroup finds the slopes of its sequences itself, from their sums and
+// their partners'; the last workgroup, which has no chunk, the loss and the rewards.
+constexpr int64_t FEW_SEQS = 2048;  // (a power of two)
+template <class T, int GROUP>
+__global__ __launch_bounds__(BLOCK) void few_slopes_kernel(Seqs q, Preference o, int64_t chunks, Space sp, typename Num<T>::acc* f, typename Num<T>::acc* rewards, T* grad) {
+    __shared__ double slope[FEW_SEQS];
+    __shared__ int64_t ends[2];
+    if (blockIdx.x == gridDim.x - 1) {
+        pair_losses<GROUP>(q, o, sp, rewards, false, 0, 1);
+        if (threadIdx.x == 0) *f = (typename Num<T>::acc)(sp.loss[0] / (double)(q.count / 2));
+        return;
+    }
+    const int64_t pairs = q.count / 2, groups = gridDim.x - 1;
+    const int l = threadIdx.x % GROUP;
+    int64_t had = -1, had_n = 0;  // adjacent chunks for a workgroup: long sequences stay the same, and what is known of them
+    const int64_t last_w = (blockIdx.x + 1) * chunks / groups;
+    for (int64_t w = blockIdx.x * chunks / groups; w < last_w; w++) {
+        const int64_t t0 = w * CHUNK + threadIdx.x * E;
+        Pack<uint8_t, E> keep;
+        load_mask(q.mask, t0, q.tokens, keep);
+        const Spot at = q.locate(t0);
+        if (threadIdx.x == 0) ends[0] = at.s;
+        if (threadIdx.x == BLOCK - 1) {  // the last sequence that begins in the chunk
+            Spot last = at;
+            while (last.end <= E) q.next(last, t0);
+            ends[1] = last.s < q.count ? last.s : q.count - 1;
+        }
+        __syncthreads();
+        const int64_t first = ends[0], n = ends[1] - first + 1;
+        const bool known = first == had && n == had_n;
+        had = first, had_n = n;
+        for (int64_t k = 0; k < n && !known; k += BLOCK / GROUP) {
+            const int64_t j = k + threadIdx.x / GROUP, s = first + j;
+            const bool real = j < n;
+            const int64_t other = !real ? 0 : s < pairs ? s + pairs : s - pairs;
+            const Rec mine = sequence<GROUP>(q, sp, real && s < 2 * pairs ? s : 0, l), its = sequence<GROUP>(q, sp, real && s < 2 * pairs ? other : 0, l);
+            if (real && s < 2 * pairs && l == 0) {
+                const bool preferred = s < pairs;
+                const Pair p = pair_of(o, preferred ? mine : its, preferred ? its : mine, q.good(s) && q.good(other), pairs);
+                slope[j] = preferred ? p.preferred : p.rejected;
+            }
+        }
+        __syncthreads();
+        chunk_slopes(q, slope, first, FEW_SEQS - 1, grad, w, at, keep);
+        __syncthreads();
+    }
+}
+// a small batch: all of it as one workgroup, with nothing between the passes but LDS
 template <class T>
-__global__ __launch_bounds__(BLOCK) void preference_small_kernel(Seqs q, Preference o, const T* a, const T* b, int64_t chunks, Space sp,
+__global__ __launch_bounds__(BLOCK) void preference_small_kernel(Seqs whole, Preference o, const T* a, const T* b, int chunks,
                                                                  typename Num<T>::acc* f, typename Num<T>::acc* rewards, T* grad) {
-    for (int64_t w = 0; w < chunks; w++) chunk_sums(q, a, b, w, sp);
+    __shared__ SmallSpace m;
+    Space sp;
+    Tokens<T> x[SMALL_CHUNKS];
+#pragma unroll
+    for (int w = 0; w < SMALL_CHUNKS; w++)
+        if (w < chunks) x[w].get(whole.mask, a, b, w * CHUNK + threadIdx.x * E, whole.tokens);
+    const SmallSeqs q = small_seqs(whole, m, sp);
     __syncthreads();
-    pair_losses(q, o, sp, rewards, 0, 1);
+#pragma unroll
+    for (int w = 0; w < SMALL_CHUNKS; w++)
+        if (w < chunks) chunk_sums(q, x[w], a != nullptr, b != nullptr, w, sp);
     __syncthreads();
-    mean_loss(sp, 1, q.count / 2, f);
-    for (int64_t w = 0; w < chunks; w++) chunk_slopes(q, sp, grad, w);
+    pair_losses<1>(q, o, sp, rewards, true, 0, 1);
+    __syncthreads();
+    if (threadIdx.x == 0) *f = (typename Num<T>::acc)(sp.loss[0] / (double)(q.count / 2));
+#pragma unroll
+    for (int w = 0; w < SMALL_CHUNKS; w++)
+        if (w < chunks) chunk_slopes(q, sp.slope, 0, -1, grad, w, q.locate(w * CHUNK + threadIdx.x * E), x[w].keep);
 }
 
 // ------------------------------------------------------------------------------------ policy
@@ -347,7 +514,8 @@ __device__ __forceinline__ void kl_terms(double q, double& em1, double& k) {
 }
 
 // tokens of each sequence that count -> 1 / their number; kept tokens and sequences with any of this workgroup
-__device__ __forceinline__ void sequence_weights(const Seqs& q, const Space& sp, int block, int blocks) {
+template <class Q>
+__device__ __forceinline__ void sequence_weights(const Q& q, const Space& sp, int block, int blocks) {
     constexpr int GROUP = 8;
     const int l = threadIdx.x % GROUP;
     const int64_t each = (int64_t)blocks * (BLOCK / GROUP), rounds = (q.count + each - 1) / each;
@@ -372,13 +540,88 @@ __device__ __forceinline__ void sequence_weights(const Seqs& q, const Space& sp,
     if (threadIdx.x == 0) sp.counts[2 * block] = kept, sp.counts[2 * block + 1] = some;
 }
 
-// the sum of both counts over the workgroups of sequence_weights (at most a wave of them), in every thread
+// the mean over all tokens needs their number alone: kept places between the first offset and the last, and whether all are good
+__global__ __launch_bounds__(BLOCK) void count_kernel(Seqs q, Space sp) {
+    constexpr int N = 16;
+    const int64_t begin = q.at(0), end = q.at(q.count), stride = (int64_t)gridDim.x * BLOCK;
+    const int64_t me = (int64_t)blockIdx.x * BLOCK + threadIdx.x;
+    int kept = 0;
+    constexpr int U = 4;
+    for (int64_t t = begin + me * N; t < end; t += stride * N * U) {
+        Pack<uint8_t, N> m[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int64_t at = t + u * stride * N;
+            if (at + N <= end)
+                m[u] = *(const Pack<uint8_t, N>*)(q.mask + at);
+            else
+#pragma unroll
+                for (int k = 0; k < N; k++) m[u].v[k] = at + k < end ? q.mask[at + k] : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int k = 0; k < N; k++) kept += m[u].v[k] != 0;
+    }
+    bool bad = false;
+    for (int64_t s = me; s < q.count; s += stride) bad |= !q.good(s);
+    const double n = block_sum((double)kept), b = block_sum(bad ? 1.0 : 0.0);
+    if (threadIdx.x == 0) sp.counts[2 * blockIdx.x] = b > 0 ? NAN : n, sp.counts[2 * blockIdx.x + 1] = 0;
+}
+
+// the sum of both counts over the workgroups that counted, in every thread
 __device__ __forceinline__ void all_counts(const Space& sp, int blocks, double& kept, double& some) {
-    const int lane = threadIdx.x % WAVE;
-    kept = wave_sum(lane < blocks ? sp.counts[2 * lane] : 0.0);
-    some = wave_sum(lane < blocks ? sp.counts[2 * lane + 1] : 0.0);
+    kept = some = 0;
+    for (int k = threadIdx.x % WAVE; k < blocks; k += WAVE) kept += sp.counts[2 * k], some += sp.counts[2 * k + 1];
+    kept = wave_sum(kept);
+    some = wave_sum(some);
     if (kept < 1) kept = 1;  // nothing counts: sums of nothing, divided by something
     if (some < 1) some = 1;
+}
+
+// e^d in 64 bits, to 2^-42: d = n log 2 + r, a polynomial of r, the power of two.  (The library's is right to the last of 53 bits,
+// which for ratios of 32-bit values nobody sees, and takes twice as long.)  Beyond the range, infinities and NaN: the library's.
+__device__ __forceinline__ double exp_of(double d) {
+    if (!(fabs(d) < 600)) return exp(d);
+    const double n = rint(d * 1.4426950408889634);
+    const double r = fma(n, -2.3190468138462996e-17, fma(n, -0.6931471805599453, d));  // log 2 and what a double leaves of it
+    double p = 1.0 / 3628800;  // the Taylor series to r^10, |r| < 0.347: the first term left out is below 2^-42 of r / 11
+    p = fma(p, r, 1.0 / 362880);
+    p = fma(p, r, 1.0 / 40320);
+    p = fma(p, r, 1.0 / 5040);
+    p = fma(p, r, 1.0 / 720);
+    p = fma(p, r, 1.0 / 120);
+    p = fma(p, r, 1.0 / 24);
+    p = fma(p, r, 1.0 / 6);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return ldexp(p, (int)n);
+}
+// Of a token's log-probabilities: r A, and whether the border that its advantage goes with is passed.  In 32 bits where that is as good
+// -- the difference itself, and r - 1 for a small one, so that r is right to 2^-22 |r - 1| -- and in 64 where it is not: at the border
+// (the gradient jumps there), and for a large difference.
+__device__ __forceinline__ void ratio(const Policy& o, float lp, float old, double a, bool& over, double& ra) {
+    const float d = lp - old;
+    const double border = a > 0 ? o.log_high : o.log_low;
+    const float b = (float)border;
+    over = a > 0 ? d > b : a < 0 && d < b;
+    if (!(fabsf(d - b) > 1e-6f * fabsf(b))) {  // (d and b are within 2^-23 of what they stand for)
+        const double e = (double)lp - (double)old;
+        over = a > 0 ? e > border : a < 0 && e < border;
+    }
+    if (fabsf(d) < 0.5f) {
+        float em1, k;
+        kl_terms(d, em1, k);
+        ra = fma((double)em1, a, a);
+    } else {
+        ra = a == 0 && d == d ? 0 : exp_of((double)lp - (double)old) * a;  // (an advantage of 0 gives 0 for any ratio, one that overflowed too)
+    }
+}
+__device__ __forceinline__ void ratio(const Policy& o, double lp, double old, double a, bool& over, double& ra) {
+    const double d = lp - old;
+    over = (a > 0 && d > o.log_high) || (a < 0 && d < o.log_low);
+    ra = a == 0 && d == d ? 0 : exp(d) * a;
 }
 
 template <class T>
@@ -386,64 +629,70 @@ struct PolicyData {
     const T *logps, *old, *ref, *adv;
     T* grad;
 };
-
-// L = -min(r A, clip(r) A) + kl (e^q - 1 - q) with r = e^d, d = logp - old, q = ref - logp.  d is the exact difference, and
-// whether r is clipped is decided by comparing d with the borders' logarithms in 64 bits: the gradient jumps there.  r is
-// taken in 64 bits too: advantages have mean 0, and the mean of r A is what is left of terms a thousand times larger.
+// a thread's tokens
 template <class T>
-__device__ __forceinline__ void chunk_policy(const Seqs& q, const Policy& o, const PolicyData<T>& x, const Space& sp, double inv, int64_t w,
-                                             double& f, double& kl, double& clipped) {
+struct PolicyTokens {
+    Pack<T, E> lp, old, ref, adv;
+    Pack<uint8_t, E> keep;
+    __device__ __forceinline__ void get(const PolicyData<T>& x, const uint8_t* mask, bool per_token, int64_t t, int64_t n) {
+        load(x.logps, t, n, lp);
+        load(x.old, t, n, old);
+        if (x.ref) load(x.ref, t, n, ref);
+        if (per_token) load(x.adv, t, n, adv);
+        load_mask(mask, t, n, keep);
+    }
+};
+
+// L = -min(r A, clip(r) A) + kl (e^q - 1 - q) with r = e^d, d = logp - old, q = ref - logp.  Products with A and sums are taken in 64
+// bits: advantages have mean 0, and the mean of r A is what is left of terms a thousand times larger.
+template <class T>
+__device__ __forceinline__ void token(const Policy& o, T lp, T old, T ref, double a, double weight, typename Num<T>::acc& slope, double& f, double& kl, double& clipped) {
+    typedef typename Num<T>::acc A;
+    bool over;
+    double ra;
+    ratio(o, (A)lp, (A)old, a, over, ra);
+    double loss = over ? -(a > 0 ? o.high : o.low) * a : -ra;
+    slope = over ? (A)0 : (A)-ra;
+    if (o.kl != 0) {
+        A em1, term;
+        kl_terms((A)ref - (A)lp, em1, term);
+        loss += o.kl * (double)term;
+        slope -= (A)o.kl * em1;
+        kl += (double)term;
+    }
+    f += loss * weight;
+    clipped += over;
+    slope *= (A)weight;
+}
+
+template <class T, class Q>
+__device__ __forceinline__ void chunk_policy(const Q& q, const Policy& o, const PolicyTokens<T>& x, const T* advantages, T* grad, const double* inverse, double inv,
+                                             int64_t w, double& f, double& kl, double& clipped) {
     typedef typename Num<T>::acc A;
     const int64_t t0 = w * CHUNK + threadIdx.x * E, n = q.tokens;
+    Spot at = q.locate(t0);
     if (t0 >= n) return;
-    Pack<T, E> lp, old, ref, adv, g;
-    Pack<uint8_t, E> keep;
-    load(x.logps, t0, n, lp);
-    load(x.old, t0, n, old);
-    if (x.ref) load(x.ref, t0, n, ref);
-    if (o.per_token) load(x.adv, t0, n, adv);
-    load_mask(q, t0, keep);
-    Walk at;
-    at.start(q, t0);
-    double a_seq = 0;
-    double weight = inv;
+    Pack<T, E> g;
+    double a_seq = 0, weight = inv;
     auto enter = [&]() {
         if (at.s < q.count) {
-            if (!o.per_token) a_seq = (double)x.adv[at.s];
-            if (o.by_sequence) weight = inv * sp.slope[at.s];
+            if (!o.per_token) a_seq = (double)advantages[at.s];
+            if (o.by_sequence) weight = inv * inverse[at.s];
         }
     };
     enter();
 #pragma unroll
     for (int k = 0; k < E; k++) {
-        const int64_t t = t0 + k;
         A slope = 0;
-        if (at.inside(t) && keep.v[k]) {
-            const double d = (double)lp.v[k] - (double)old.v[k];
-            const double a = o.per_token ? (double)adv.v[k] : a_seq;
-            const bool over = (a > 0 && d > o.log_high) || (a < 0 && d < o.log_low);
-            // (an advantage of 0 gives 0 for any ratio, one that overflowed too)
-            const double ra = a == 0 && d == d ? 0 : exp(d) * a;
-            double loss = over ? -(a > 0 ? o.high : o.low) * a : -ra;
-            slope = over ? (A)0 : (A)-ra;
-            if (o.kl != 0) {
-                A em1, term;
-                kl_terms((A)((double)ref.v[k] - (double)lp.v[k]), em1, term);
-                loss += o.kl * (double)term;
-                slope -= (A)o.kl * em1;
-                kl += (double)term;
-            }
-            f += loss * weight;
-            clipped += over;
-            slope *= (A)weight;
-        }
+        if (k >= at.begin && k < at.end && x.keep.v[k])
+            token<T>(o, x.lp.v[k], x.old.v[k], x.ref.v[k], o.per_token ? (double)x.adv.v[k] : a_seq, weight, slope, f, kl, clipped);
         g.v[k] = (T)slope;
-        if (t + 1 == at.end) {
-            at.next(q);
+        if (k + 1 == at.end) {
+            q.next(at, t0);
             if (k + 1 < E) enter();
         }
     }
-    store(x.grad, t0, n, g);
+    store(grad, t0, n, g);
 }
 
 template <class A>
@@ -460,11 +709,54 @@ __global__ __launch_bounds__(BLOCK) void policy_kernel(Seqs q, Policy o, PolicyD
     double kept, some, f = 0, kl = 0, clipped = 0;
     all_counts(sp, count_blocks, kept, some);
     const double inv = 1.0 / (o.by_sequence ? some : kept);
-    for (int64_t w = blockIdx.x; w < chunks; w += gridDim.x) chunk_policy(q, o, x, sp, inv, w, f, kl, clipped);
+    for (int64_t w = blockIdx.x; w < chunks; w += gridDim.x) {
+        PolicyTokens<T> t;
+        t.get(x, q.mask, o.per_token, w * CHUNK + threadIdx.x * E, q.tokens);
+        chunk_policy(q, o, t, x.adv, x.grad, sp.slope, inv, w, f, kl, clipped);
+    }
     f = block_sum(f);
     kl = block_sum(kl);
     clipped = block_sum(clipped);
     if (threadIdx.x == 0) sp.sums[3 * blockIdx.x] = f, sp.sums[3 * blockIdx.x + 1] = kl, sp.sums[3 * blockIdx.x + 2] = clipped;
+}
+// The mean over all tokens with an advantage for each: nothing is a sequence's own, all tokens from the first offset to the last are
+// alike, and nobody looks for their sequences.  One pack of 16 bytes of each tensor a thread.
+constexpr int ALIKE_BLOCKS = 1280;  // five to a compute unit
+template <class T>
+__global__ __launch_bounds__(BLOCK) void policy_alike_kernel(Seqs q, Policy o, PolicyData<T> x, int count_blocks, Space sp) {
+    typedef typename Num<T>::acc A;
+    constexpr int N = vec_len<T>();
+    double kept, some, f = 0, kl = 0, clipped = 0;
+    all_counts(sp, count_blocks, kept, some);
+    const double inv = 1.0 / kept;
+    const int64_t begin = q.at(0), end = q.at(q.count), n = q.tokens, stride = (int64_t)gridDim.x * BLOCK * N;
+    for (int64_t t = ((int64_t)blockIdx.x * BLOCK + threadIdx.x) * N; t < n; t += stride) {
+        Pack<T, N> lp, old, ref, adv, g;
+        Pack<uint8_t, N> keep;
+        if (t + N <= n) {
+            lp = *(const Pack<T, N>*)(x.logps + t), old = *(const Pack<T, N>*)(x.old + t), adv = *(const Pack<T, N>*)(x.adv + t);
+            if (x.ref) ref = *(const Pack<T, N>*)(x.ref + t);
+            if (q.mask) keep = *(const Pack<uint8_t, N>*)(q.mask + t);
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                A slope = 0;
+                if (t + k >= begin && t + k < end && (!q.mask || keep.v[k])) token<T>(o, lp.v[k], old.v[k], ref.v[k], (double)adv.v[k], 1.0, slope, f, kl, clipped);
+                g.v[k] = (T)(slope * (A)inv);
+            }
+            *(Pack<T, N>*)(x.grad + t) = g;
+        } else {
+            for (int64_t k = t; k < n; k++) {
+                A slope = 0;
+                if (k >= begin && k < end && (!q.mask || q.mask[k]))
+                    token<T>(o, x.logps[k], x.old[k], x.ref ? x.ref[k] : (T)0, (double)x.adv[k], 1.0, slope, f, kl, clipped);
+                x.grad[k] = (T)(slope * (A)inv);
+            }
+        }
+    }
+    f = block_sum(f);
+    kl = block_sum(kl);
+    clipped = block_sum(clipped);
+    if (threadIdx.x == 0) sp.sums[3 * blockIdx.x] = f * inv, sp.sums[3 * blockIdx.x + 1] = kl, sp.sums[3 * blockIdx.x + 2] = clipped;
 }
 template <class A>
 __global__ __launch_bounds__(BLOCK) void policy_results_kernel(Space sp, int count_blocks, int blocks, A* out_f, A* out_kl, A* out_clipped) {
@@ -474,23 +766,40 @@ __global__ __launch_bounds__(BLOCK) void policy_results_kernel(Space sp, int cou
     policy_results(f, kl, clipped, kept, out_f, out_kl, out_clipped);
 }
 template <class T>
-__global__ __launch_bounds__(BLOCK) void policy_small_kernel(Seqs q, Policy o, PolicyData<T> x, int64_t chunks, Space sp, typename Num<T>::acc* out_f,
+__global__ __launch_bounds__(BLOCK) void policy_small_kernel(Seqs whole, Policy o, PolicyData<T> x, int chunks, typename Num<T>::acc* out_f,
                                                              typename Num<T>::acc* out_kl, typename Num<T>::acc* out_clipped) {
-    if (q.mask)
-        for (int64_t w = 0; w < chunks; w++) chunk_sums<T>(q, nullptr, nullptr, w, sp);
+    __shared__ SmallSpace m;
+    Space sp;
+    PolicyTokens<T> t[SMALL_CHUNKS];
+#pragma unroll
+    for (int w = 0; w < SMALL_CHUNKS; w++)
+        if (w < chunks) t[w].get(x, whole.mask, o.per_token, w * CHUNK + threadIdx.x * E, whole.tokens);
+    const SmallSeqs q = small_seqs(whole, m, sp);
     __syncthreads();
+    if (q.mask) {
+#pragma unroll
+        for (int w = 0; w < SMALL_CHUNKS; w++)
+            if (w < chunks) {
+                Tokens<T> k;
+                k.keep = t[w].keep;
+                chunk_sums(q, k, false, false, w, sp);
+            }
+        __syncthreads();
+    }
     sequence_weights(q, sp, 0, 1);
     __syncthreads();
     double kept, some, f = 0, kl = 0, clipped = 0;
     all_counts(sp, 1, kept, some);
     const double inv = 1.0 / (o.by_sequence ? some : kept);
-    for (int64_t w = 0; w < chunks; w++) chunk_policy(q, o, x, sp, inv, w, f, kl, clipped);
+#pragma unroll
+    for (int w = 0; w < SMALL_CHUNKS; w++)
+        if (w < chunks) chunk_policy(q, o, t[w], x.adv, x.grad, sp.slope, inv, w, f, kl, clipped);
     policy_results(f, kl, clipped, kept, out_f, out_kl, out_clipped);
 }
 
 // ------------------------------------------------------------------------------------ launches
-// up to so many tokens and sequences one workgroup does the whole of a loss
-constexpr int64_t SMALL_TOKENS = 2 * CHUNK, SMALL_SEQS = 256;
+// up to so many tokens and sequences one workgroup does the whole of a loss, without a workspace
+static bool small(int64_t tokens, int64_t seqs) { return tokens <= SMALL_TOKENS && seqs <= SMALL_SEQS; }
 
 static int64_t chunks_of(int64_t tokens) { return (tokens + CHUNK - 1) / CHUNK; }
 
@@ -518,15 +827,28 @@ template <class T>
 static void launch_preference(const Seqs& q, const Preference& o, const void* a, const void* b, void* f, void* rewards, void* grad, const Space& sp, hipStream_t s) {
     typedef typename Num<T>::acc A;
     const int64_t chunks = chunks_of(q.tokens), pairs = q.count / 2;
-    if (q.tokens <= SMALL_TOKENS && q.count <= SMALL_SEQS) {
-        preference_small_kernel<T><<<1, BLOCK, 0, s>>>(q, o, (const T*)a, (const T*)b, chunks, sp, (A*)f, (A*)rewards, (T*)grad);
+    if (small(q.tokens, q.count)) {
+        preference_small_kernel<T><<<1, BLOCK, 0, s>>>(q, o, (const T*)a, (const T*)b, (int)chunks, (A*)f, (A*)rewards, (T*)grad);
         return;
     }
-    const int64_t groups = (pairs * 8 + BLOCK - 1) / BLOCK;
+    // the records of a sequence (one for each chunk it reaches) are added up by one lane, or by eight where there are many
+    const bool many = q.tokens / q.count > 4 * CHUNK;
+    const int64_t groups = (pairs * (many ? 8 : 1) + BLOCK - 1) / BLOCK;
     const int blocks = (int)(groups < LOSS_BLOCKS ? groups : LOSS_BLOCKS);
     const unsigned grid = (unsigned)(chunks < (1 << 20) ? (chunks ? chunks : 1) : (1 << 20));
     if (chunks) sums_kernel<T><<<grid, BLOCK, 0, s>>>(q, (const T*)a, (const T*)b, chunks, sp);
-    pairs_kernel<A><<<blocks, BLOCK, 0, s>>>(q, o, sp, (A*)rewards);
+    if (q.count <= FEW_SEQS) {
+        const unsigned grid = (unsigned)(chunks < 768 ? chunks : 768);  // (three to a compute unit: all of them at once)
+        if (many)
+            few_slopes_kernel<T, 8><<<grid + 1, BLOCK, 0, s>>>(q, o, chunks, sp, (A*)f, (A*)rewards, (T*)grad);
+        else
+            few_slopes_kernel<T, 1><<<grid + 1, BLOCK, 0, s>>>(q, o, chunks, sp, (A*)f, (A*)rewards, (T*)grad);
+        return;
+    }
+    if (many)
+        pairs_kernel<8, A><<<blocks, BLOCK, 0, s>>>(q, o, sp, (A*)rewards);
+    else
+        pairs_kernel<1, A><<<blocks, BLOCK, 0, s>>>(q, o, sp, (A*)rewards);
     slopes_kernel<T><<<grid, BLOCK, 0, s>>>(q, chunks, blocks, sp, (A*)f, (T*)grad);
 }
 
@@ -536,16 +858,27 @@ static void launch_policy(const Seqs& q, const Policy& o, const void* logps, con
     typedef typename Num<T>::acc A;
     const int64_t chunks = chunks_of(q.tokens);
     const PolicyData<T> x = {(const T*)logps, (const T*)old, (const T*)ref, (const T*)adv, (T*)grad};
-    if (q.tokens <= SMALL_TOKENS && q.count <= SMALL_SEQS) {
-        policy_small_kernel<T><<<1, BLOCK, 0, s>>>(q, o, x, chunks, sp, (A*)f, (A*)kl, (A*)clipped);
+    if (small(q.tokens, q.count)) {
+        policy_small_kernel<T><<<1, BLOCK, 0, s>>>(q, o, x, (int)chunks, (A*)f, (A*)kl, (A*)clipped);
         return;
     }
-    const int64_t groups = (q.count * 8 + BLOCK - 1) / BLOCK;
+    const bool total = q.mask && !o.by_sequence;  // the number of all tokens is wanted, not each sequence's
+    const int64_t groups = total ? (q.tokens + 16 * BLOCK - 1) / (16 * BLOCK) + 1 : (q.count * 8 + BLOCK - 1) / BLOCK;
     const int count_blocks = (int)(groups < COUNT_BLOCKS ? groups : COUNT_BLOCKS);
-    const int blocks = (int)(chunks < POLICY_BLOCKS ? (chunks ? chunks : 1) : POLICY_BLOCKS);
-    if (q.mask && chunks) sums_kernel<T><<<(unsigned)(chunks < (1 << 20) ? chunks : (1 << 20)), BLOCK, 0, s>>>(q, (const T*)nullptr, (const T*)nullptr, chunks, sp);
-    weights_kernel<<<count_blocks, BLOCK, 0, s>>>(q, sp);
-    policy_kernel<T><<<blocks, BLOCK, 0, s>>>(q, o, x, chunks, count_blocks, sp);
+    int blocks = (int)(chunks < POLICY_BLOCKS ? (chunks ? chunks : 1) : POLICY_BLOCKS);
+    if (total) {
+        count_kernel<<<count_blocks, BLOCK, 0, s>>>(q, sp);
+    } else {
+        if (q.mask && chunks) sums_kernel<T><<<(unsigned)(chunks < (1 << 20) ? chunks : (1 << 20)), BLOCK, 0, s>>>(q, (const T*)nullptr, (const T*)nullptr, chunks, sp);
+        weights_kernel<<<count_blocks, BLOCK, 0, s>>>(q, sp);
+    }
+    if (o.per_token && !o.by_sequence) {
+        const int64_t packs = (q.tokens + vec_len<T>() - 1) / vec_len<T>(), need = (packs + BLOCK - 1) / BLOCK;
+        blocks = (int)(need < ALIKE_BLOCKS ? (need ? need : 1) : ALIKE_BLOCKS);
+        policy_alike_kernel<T><<<blocks, BLOCK, 0, s>>>(q, o, x, count_blocks, sp);
+    } else {
+        policy_kernel<T><<<blocks, BLOCK, 0, s>>>(q, o, x, chunks, count_blocks, sp);
+    }
     policy_results_kernel<A><<<1, BLOCK, 0, s>>>(sp, count_blocks, blocks, (A*)f, (A*)kl, (A*)clipped);
 }
 
@@ -564,7 +897,9 @@ static int check_seqs(const lbfgs_train_sequences* in, Seqs* q, const char* who)
     return LBFGS_HIP_OK;
 }
 static int check_workspace(const void* workspace, uint64_t bytes, const Seqs& q, Space* sp, const char* who) {
-    const uint64_t need = lay_out(nullptr, nullptr, q.tokens, q.count);
+    const uint64_t need = lbfgs_train_sequences_workspace(q.tokens, q.count);
+    *sp = Space();
+    if (!need) return LBFGS_HIP_OK;
     if (!workspace || bytes < need)
         return lt_fail(LBFGS_HIP_ERR_ARG, "%s: %llu bytes of workspace, %llu are needed", who, (unsigned long long)(workspace ? bytes : 0), (unsigned long long)need);
     lay_out(sp, (void*)workspace, q.tokens, q.count);
@@ -601,7 +936,7 @@ extern "C" const char* lbfgs_train_last_error(void) { return g_error; }
 
 extern "C" uint64_t lbfgs_train_sequences_workspace(int64_t tokens, int64_t count) {
     if (tokens < 0 || count < 1 || tokens > (INT64_MAX >> 20) || count > (INT64_MAX >> 20)) return 0;
-    return lay_out(nullptr, nullptr, tokens, count);
+    return small(tokens, count) ? 0 : lay_out(nullptr, nullptr, tokens, count);
 }
 
 extern "C" int lbfgs_train_preference(const lbfgs_train_sequences* seqs, const void* logps, const void* ref_logps, double beta, double label_smoothing,

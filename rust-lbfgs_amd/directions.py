@@ -30,15 +30,14 @@ def orthogonalize(update, *, steps=5, coefficients=COEFFICIENTS):
         raise ValueError(f"update must be [..., rows, cols], not {tuple(update.shape)}")
     if len(coefficients) != 3:
         raise ValueError(f"coefficients are (a, b, c), not {coefficients!r}")
-    dev = _train.on_gpu(("update", update))
+    dev = _train.on_gpu("update", update)
     L = _train.load()
-    with _train.current(dev):
-        g = update.detach().contiguous()
-        out = torch.empty_like(g)
-        rows, cols = g.shape[-2:]
-        batch = g.numel() // (rows * cols) if rows and cols else 0
-        size = L.lbfgs_train_orthogonalize_workspace(_train.DTYPES[g.dtype], batch, rows, cols)
-        ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-        _train.check(L.lbfgs_train_orthogonalize(_train.DTYPES[g.dtype], batch, rows, cols, g.data_ptr(), out.data_ptr(), steps, *coefficients,
-                                                 _train.ptr(ws), size, _train.stream_of(dev)))
+    g = update if update.is_contiguous() else update.detach().contiguous()
+    out = torch.empty(g.shape, dtype=g.dtype, device=dev)
+    rows, cols = g.shape[-2:]
+    batch = g.numel() // (rows * cols) if rows and cols else 0
+    size = L.lbfgs_train_orthogonalize_workspace(_train.DTYPES[g.dtype], batch, rows, cols)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    _train.enqueue(L.lbfgs_train_orthogonalize, dev, _train.DTYPES[g.dtype], batch, rows, cols, g.data_ptr(), out.data_ptr(), steps, *coefficients,
+                   _train.ptr(ws), size)
     return out

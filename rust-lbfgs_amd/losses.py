@@ -16,7 +16,6 @@ Kernels: rust-lbfgs_amd/csrc/train/{logprobs,losses}.hip behind include/lbfgs_tr
 from __future__ import annotations
 
 import ctypes as C
-import math
 from typing import NamedTuple
 
 import torch
@@ -30,7 +29,7 @@ REDUCTIONS = {"tokens": 0, "sequences": 1}
 
 # ------------------------------------------------------------------------------------ token log-probabilities
 def _rows(logits, targets, ignore_index):
-    """-> (Rows, what keeps its memory alive).  A view without its last positions ([:, :-1]) is read as it is."""
+    """-> (Rows, device, what keeps its memory alive).  A view without its last positions ([:, :-1]) is read as it is."""
     _train.floating("logits", logits)
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"logits must be [..., vocabulary] with at least one entry, not {tuple(logits.shape)}")
@@ -38,18 +37,22 @@ def _rows(logits, targets, ignore_index):
         raise TypeError(f"targets must be an int64 tensor, not {getattr(targets, 'dtype', type(targets).__name__)}")
     if targets.shape != logits.shape[:-1]:
         raise ValueError(f"targets must have shape {tuple(logits.shape[:-1])}, one for each row of logits, not {tuple(targets.shape)}")
-    _train.on_gpu(("logits", logits), targets=targets)
-    targets = targets.contiguous()
-    x = logits.detach()
-    if x.dim() > 3:
-        x = x.flatten(0, -3)  # (a copy only if the leading dimensions have no common stride)
-    while x.dim() < 3:
-        x = x.unsqueeze(0)
-    if (x.shape[-1] > 1 and x.stride(-1) != 1) or any(n > 1 and st < 0 for n, st in zip(x.shape, x.stride())):
-        x = x.contiguous()
-    r = _train.Rows(x.data_ptr(), targets.data_ptr(), _train.DTYPES[x.dtype], 0, x.shape[0], x.shape[1], x.shape[2], x.stride(0), x.stride(1),
-                    int(ignore_index))
-    return r, (x, targets)
+    dev = _train.on_gpu("logits", logits, (("targets", targets),))
+    if not targets.is_contiguous():
+        targets = targets.contiguous()
+    x = logits
+    n = x.dim()
+    if n > 3:
+        x = x.detach().flatten(0, -3)  # (a copy only if the leading dimensions have no common stride)
+        n = 3
+    shape, strides = x.shape, x.stride()
+    if (shape[-1] > 1 and strides[-1] != 1) or min(strides) < 0:
+        x = x.detach().contiguous()
+        strides = x.stride()
+    outer, outer_stride = (shape[0], strides[0]) if n == 3 else (1, 0)
+    inner, inner_stride = (shape[-2], strides[-2]) if n > 1 else (1, 0)
+    r = _train.Rows(x.data_ptr(), targets.data_ptr(), _train.DTYPES[x.dtype], 0, outer, inner, shape[-1], outer_stride, inner_stride, ignore_index)
+    return r, dev, (x, targets)
 
 
 def token_logprobs_with_lse(logits, targets, temperature=1.0, ignore_index=-100):
@@ -59,15 +62,13 @@ def token_logprobs_with_lse(logits, targets, temperature=1.0, ignore_index=-100)
     -> (logps [...] in float64 for float64 logits, else float32; lse [..., 2] float64: each row's largest logit m and
     log sum exp((logits - m) / temperature), the two parts of its log-sum-exp m / temperature + that).  A target `ignore_index` gives 0 and its
     row is not read; any other target outside [0, V) gives NaN.  Masked logits may be -inf or the type's lowest value."""
-    rows, keep = _rows(logits, targets, ignore_index)
-    L, dev = _train.load(), logits.device
-    with _train.current(dev):
-        logps = torch.empty(targets.shape, dtype=_train.wide(logits.dtype), device=dev)
-        lse = torch.empty((*targets.shape, 2), dtype=torch.float64, device=dev)
-        size = L.lbfgs_train_token_logprobs_workspace(rows.dtype, targets.numel(), rows.vocab)
-        ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-        _train.check(L.lbfgs_train_token_logprobs(C.byref(rows), temperature, logps.data_ptr(), lse.data_ptr(), _train.ptr(ws), size,
-                                                  _train.stream_of(dev)))
+    rows, dev, keep = _rows(logits, targets, ignore_index)
+    L = _train.load()
+    logps = torch.empty(targets.shape, dtype=_train.wide(logits.dtype), device=dev)
+    lse = torch.empty((*targets.shape, 2), dtype=torch.float64, device=dev)
+    size = L.lbfgs_train_token_logprobs_workspace(rows.dtype, rows.outer * rows.inner, rows.vocab)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    _train.enqueue(L.lbfgs_train_token_logprobs, dev, C.byref(rows), temperature, logps.data_ptr(), lse.data_ptr(), _train.ptr(ws), size)
     del keep
     return logps, lse
 
@@ -77,16 +78,14 @@ def token_logprobs_grad(logits, targets, lse, grad, temperature=1.0, ignore_inde
 
     `lse` and the other arguments are those of token_logprobs_with_lse; `grad` [...] is df/dlogps in its type.  Rows whose
     grad is 0 are not read."""
-    rows, keep = _rows(logits, targets, ignore_index)
-    _train.like("lse", lse, "the logits", logits, torch.float64, (*targets.shape, 2))
-    _train.like("grad", grad, "the logits", logits, _train.wide(logits.dtype), targets.shape)
-    dev = _train.on_gpu(("logits", logits), lse=lse, grad=grad)
+    rows, dev, keep = _rows(logits, targets, ignore_index)
+    _train.like("lse", lse, "logits", torch.float64, (*targets.shape, 2))
+    _train.like("grad", grad, "logits", _train.wide(logits.dtype), targets.shape)
+    _train.on_gpu("logits", logits, (("lse", lse), ("grad", grad)))
     L = _train.load()
-    with _train.current(dev):
-        lse, grad = lse.contiguous(), grad.contiguous()
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-        _train.check(L.lbfgs_train_token_logprobs_grad(C.byref(rows), temperature, lse.data_ptr(), grad.data_ptr(), out.data_ptr(),
-                                                       _train.stream_of(dev)))
+    lse, grad = lse.contiguous(), grad.contiguous()
+    out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    _train.enqueue(L.lbfgs_train_token_logprobs_grad, dev, C.byref(rows), temperature, lse.data_ptr(), grad.data_ptr(), out.data_ptr())
     del keep
     return out
 
@@ -116,30 +115,34 @@ def token_logprobs(logits, targets, temperature=1.0, ignore_index=-100):
 
 
 # ------------------------------------------------------------------------------------ losses over sequences
+def _dense(t):
+    return t if t is None or t.is_contiguous() else t.detach().contiguous()
+
+
 def _sequences(logps, offsets, mask, others):
     """-> (Sequences, number of them, the tensors, dense, in the order logps, mask, offsets, others)."""
     _train.floating("logps", logps)
-    for name, t in others.items():
+    shape, dtype = logps.shape, logps.dtype
+    for name, t in others:
         if t is not None:
-            _train.like(name, t, "logps", logps)
+            _train.like(name, t, "logps", dtype, shape)
     if mask is not None:
-        _train.like("mask", mask, "logps", logps, torch.bool)
+        _train.like("mask", mask, "logps", torch.bool, shape)
     if offsets is None:
-        if logps.dim() != 2 or logps.shape[0] < 1:
-            raise ValueError(f"without offsets logps must be a padded batch [sequences, tokens], not {tuple(logps.shape)}")
-        count = logps.shape[0]
+        if len(shape) != 2 or shape[0] < 1:
+            raise ValueError(f"without offsets logps must be a padded batch [sequences, tokens], not {tuple(shape)}")
+        count, bits = shape[0], 0
     else:
         if not isinstance(offsets, torch.Tensor) or offsets.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"offsets must be an int32 or int64 tensor, not {getattr(offsets, 'dtype', type(offsets).__name__)}")
         if offsets.dim() != 1 or offsets.shape[0] < 2:
             raise ValueError(f"offsets must be [sequences + 1], not {tuple(offsets.shape)}")
-        if logps.dim() != 1:
-            raise ValueError(f"with offsets logps must be one-dimensional, not {tuple(logps.shape)}")
-        count = offsets.shape[0] - 1
-    dense = [t if t is None else t.detach().contiguous() for t in (logps, mask, offsets, *others.values())]
-    bits = 0 if offsets is None else 32 if offsets.dtype == torch.int32 else 64
-    q = _train.Sequences(_train.ptr(dense[2]), _train.ptr(dense[1]), bits, _train.DTYPES[logps.dtype], logps.numel(), count)
-    return q, count, dense
+        if len(shape) != 1:
+            raise ValueError(f"with offsets logps must be one-dimensional, not {tuple(shape)}")
+        count, bits = offsets.shape[0] - 1, 32 if offsets.dtype == torch.int32 else 64
+    x, m, o = _dense(logps), _dense(mask), _dense(offsets)
+    q = _train.Sequences(_train.ptr(o), _train.ptr(m), bits, _train.DTYPES[dtype], x.numel(), count)
+    return q, count, (x, m, o, *[_dense(t) for _, t in others])
 
 
 class Preference(NamedTuple):
@@ -158,17 +161,16 @@ def preference(logps, ref_logps=None, *, offsets=None, mask=None, beta=0.1, kind
     All sums are taken in 64 bits.  -> Preference(f, rewards, grad); f and rewards in float64 for float64 data, else float32."""
     if kind not in KINDS:
         raise ValueError(f"kind must be one of {', '.join(KINDS)}, not {kind!r}")
-    q, count, (x, m, o, ref) = _sequences(logps, offsets, mask, {"ref_logps": ref_logps})
-    dev = _train.on_gpu(("logps", logps), offsets=offsets, mask=mask, ref_logps=ref_logps)
-    L = _train.load()
-    with _train.current(dev):
-        out = _train.wide(x.dtype)
-        f, rewards = torch.empty((), dtype=out, device=dev), torch.empty(count, dtype=out, device=dev)
-        grad = torch.empty_like(x)
-        size = L.lbfgs_train_sequences_workspace(q.tokens, count)
-        ws = torch.empty(size, dtype=torch.uint8, device=dev)
-        _train.check(L.lbfgs_train_preference(C.byref(q), x.data_ptr(), _train.ptr(ref), beta, label_smoothing, KINDS[kind], int(normalize_lengths),
-                                              f.data_ptr(), rewards.data_ptr(), grad.data_ptr(), ws.data_ptr(), size, _train.stream_of(dev)))
+    others = (("ref_logps", ref_logps),)
+    q, count, (x, m, o, ref) = _sequences(logps, offsets, mask, others)
+    dev = _train.on_gpu("logps", logps, (("offsets", offsets), ("mask", mask), *others))
+    L, out = _train.load(), _train.wide(x.dtype)
+    f, rewards = torch.empty((), dtype=out, device=dev), torch.empty(count, dtype=out, device=dev)
+    grad = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    size = L.lbfgs_train_sequences_workspace(q.tokens, count)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    _train.enqueue(L.lbfgs_train_preference, dev, C.byref(q), x.data_ptr(), _train.ptr(ref), beta, label_smoothing, KINDS[kind], bool(normalize_lengths),
+                   f.data_ptr(), rewards.data_ptr(), grad.data_ptr(), _train.ptr(ws), size)
     return Preference(f, rewards, grad)
 
 
@@ -190,20 +192,18 @@ def policy(logps, old_logps, advantages, *, ref_logps=None, offsets=None, mask=N
         raise ValueError(f"reduction must be one of {', '.join(REDUCTIONS)}, not {reduction!r}")
     if kl_coef != 0 and ref_logps is None:
         raise ValueError("a KL term needs ref_logps")
-    q, count, (x, m, o, old, ref) = _sequences(logps, offsets, mask, {"old_logps": old_logps, "ref_logps": ref_logps})
-    per_token = not (isinstance(advantages, torch.Tensor) and tuple(advantages.shape) == (count, 1))
-    _train.like("advantages", advantages, "logps (or [sequences, 1])", logps, shape=None if per_token else (count, 1))
-    dev = _train.on_gpu(("logps", logps), offsets=offsets, mask=mask, old_logps=old_logps, advantages=advantages, ref_logps=ref_logps)
-    L = _train.load()
-    with _train.current(dev):
-        adv = advantages.detach().contiguous()
-        f, kl, clipped = torch.empty(3, dtype=_train.wide(x.dtype), device=dev).unbind()
-        grad = torch.empty_like(x)
-        size = L.lbfgs_train_sequences_workspace(q.tokens, count)
-        ws = torch.empty(size, dtype=torch.uint8, device=dev)
-        _train.check(L.lbfgs_train_policy(C.byref(q), x.data_ptr(), old.data_ptr(), _train.ptr(ref), adv.data_ptr(), int(per_token), clip_low, clip_high,
-                                          kl_coef, REDUCTIONS[reduction], f.data_ptr(), kl.data_ptr(), clipped.data_ptr(), grad.data_ptr(), ws.data_ptr(),
-                                          size, _train.stream_of(dev)))
+    others = (("old_logps", old_logps), ("ref_logps", ref_logps))
+    q, count, (x, m, o, old, ref) = _sequences(logps, offsets, mask, others)
+    per_token = not (isinstance(advantages, torch.Tensor) and advantages.shape == (count, 1))
+    _train.like("advantages", advantages, "logps (or [sequences, 1])", x.dtype, x.shape if per_token else (count, 1))
+    dev = _train.on_gpu("logps", logps, (("offsets", offsets), ("mask", mask), ("advantages", advantages), *others))
+    L, adv = _train.load(), _dense(advantages)
+    f, kl, clipped = torch.empty(3, dtype=_train.wide(x.dtype), device=dev).unbind()
+    grad = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    size = L.lbfgs_train_sequences_workspace(q.tokens, count)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    _train.enqueue(L.lbfgs_train_policy, dev, C.byref(q), x.data_ptr(), old.data_ptr(), _train.ptr(ref), adv.data_ptr(), per_token, clip_low, clip_high, kl_coef,
+                   REDUCTIONS[reduction], f.data_ptr(), kl.data_ptr(), clipped.data_ptr(), grad.data_ptr(), _train.ptr(ws), size)
     return Policy(f, kl, clipped, grad)
 
 

@@ -339,7 +339,7 @@ def policy_in_64_bits(lp, old, adv, ref, spans, keep, low, high, kl_coef, reduct
     parts = torch.zeros_like(old)
     parts[keep] = ((torch.where(over, 0.0, r * a).abs() + abs(kl_coef) * (1 + q.exp())) * w[keep]).detach()
     return (f.detach(), k3.detach().sum() / N, over.double().sum() / N, grad, parts, (loss.abs() * w[keep]).detach().sum(),
-            abs(kl_coef) * (k3 * w[keep]).detach().sum())
+            abs(kl_coef) * (k3 * w[keep]).detach().sum(), (torch.where(over, 0.0, (r - 1) * a).abs() * w[keep]).detach().sum())
 
 
 @pytest.mark.parametrize("dtype", DT)
@@ -357,10 +357,11 @@ def test_policy(lengths, layout, dtype):
         adv.reshape(-1)[::7] = 0
         low, high = (0.2, 0.28) if k % 2 else (0.1, 0.1)
         got = losses.policy(lp, old, adv, ref_logps=ref, offsets=off, mask=mask, clip_low=low, clip_high=high, kl_coef=kl_coef, reduction=reduction)
-        f, kl, clip, grad, parts, size, klsize = policy_in_64_bits(lp, old, adv, ref, spans, keep, low, high, kl_coef, reduction)
+        f, kl, clip, grad, parts, size, klsize, beyond = policy_in_64_bits(lp, old, adv, ref, spans, keep, low, high, kl_coef, reduction)
         what = (lengths, layout, dtype, reduction, kl_coef)
-        # f: its KL part has 32-bit terms (10 roundings each), the rest and all sums are 64-bit
-        near(got.f, f, u * f.abs() + 10 * u * klsize + 1e-14 * size, what)
+        # f: its KL part has 32-bit terms (10 roundings each), and so has r - 1 (the difference's rounding, the series' four); products
+        # with the advantage and all sums are 64-bit
+        near(got.f, f, u * f.abs() + 10 * u * klsize + 6 * u * beyond + 1e-14 * size, what)
         near(got.kl, kl, 11 * u * kl.abs(), what)
         near(got.clip_fraction, clip, u * clip, what)
         # grad: advantage's product, KL term, their sum, the weight and its product

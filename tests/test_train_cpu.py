@@ -125,9 +125,10 @@ def test_c_preference_refusals(lib):
     refused(call(kind=3), "kind")
     for name in ("logps", "f", "rewards", "grad"):
         refused(call(**{name: None}), "are needed")
-    need = lib.lbfgs_train_sequences_workspace(10, 4)
-    refused(call(size=need - 1), "workspace")
-    refused(call(ws=None), "workspace")
+    assert lib.lbfgs_train_sequences_workspace(10, 4) == 0 and call(seqs(count=3), ws=None, size=0) == ARG
+    need = lib.lbfgs_train_sequences_workspace(100000, 4)
+    refused(call(seqs(tokens=100000), size=need - 1), "workspace")
+    refused(call(seqs(tokens=100000), ws=None), "workspace")
 
 
 def test_c_policy_refusals(lib):
@@ -142,7 +143,7 @@ def test_c_policy_refusals(lib):
     refused(call(ref=None), "ref_logps")
     for name in ("logps", "old", "adv", "f", "kl", "clip", "grad"):
         refused(call(**{name: None}), "are needed")
-    refused(call(size=10), "workspace")
+    refused(call(seqs(tokens=100000), size=10), "workspace")
 
 
 def test_c_orthogonalize_refusals(lib):
