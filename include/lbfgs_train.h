@@ -104,7 +104,7 @@ int lbfgs_train_policy(const lbfgs_train_sequences* seqs, const void* logps, con
 /* ------------------------------------------------------------------------- */
 /* the matrix form of an update                                                */
 /* ------------------------------------------------------------------------- */
-/* `batch` dense matrices rows x cols (F32, BF16, F16; batch <= 65535, sides <= 2^20): each is divided by its Frobenius norm (a
+/* `batch` dense matrices rows x cols (F32, BF16, F16; batch <= 32767, sides <= 2^20): each is divided by its Frobenius norm (a
  * matrix of zeros stays one), and then `steps` times every singular value s becomes a s + b s^3 + c s^5, the singular vectors
  * staying as they are:  X <- (a I + b S + c S S) X, S = X X^T, in products of 32-bit precision.  Coefficients that lead a
  * singular value of [0, 1] beyond 64, or multiply one by more than 16384 in all, are refused. */

@@ -587,7 +587,7 @@ static void launch_orthogonalize(const Plan& q, const void* g, void* out, const 
 using namespace lt;
 
 extern "C" uint64_t lbfgs_train_orthogonalize_workspace(int32_t dtype, int64_t batch, int64_t rows, int64_t cols) {
-    if (dtype < LBFGS_TRAIN_F32 || dtype > LBFGS_TRAIN_F16 || batch < 1 || rows < 1 || cols < 1 || batch > 65535 || rows > (1 << 20) || cols > (1 << 20)) return 0;
+    if (dtype < LBFGS_TRAIN_F32 || dtype > LBFGS_TRAIN_F16 || batch < 1 || rows < 1 || cols < 1 || batch > 32767 || rows > (1 << 20) || cols > (1 << 20)) return 0;
     return lay_out(nullptr, nullptr, dtype, batch, rows, cols);
 }
 
@@ -596,7 +596,7 @@ extern "C" int lbfgs_train_orthogonalize(int32_t dtype, int64_t batch, int64_t r
     const char* who = "lbfgs_train_orthogonalize";
     if (dtype < LBFGS_TRAIN_F32 || dtype > LBFGS_TRAIN_F16)
         return lt_fail(LBFGS_HIP_ERR_ARG, "%s: element type %d: float32, bfloat16 and float16 are offered", who, dtype);
-    if (batch < 0 || rows < 0 || cols < 0 || batch > 65535 || rows > (1 << 20) || cols > (1 << 20))
+    if (batch < 0 || rows < 0 || cols < 0 || batch > 32767 || rows > (1 << 20) || cols > (1 << 20))
         return lt_fail(LBFGS_HIP_ERR_ARG, "%s: %lld matrices of %lld x %lld", who, (long long)batch, (long long)rows, (long long)cols);
     if (steps < 1 || steps > 64) return lt_fail(LBFGS_HIP_ERR_ARG, "%s: %d steps: 1 to 64 are offered", who, steps);
     if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return lt_fail(LBFGS_HIP_ERR_ARG, "%s: coefficients %g, %g, %g", who, a, b, c);

@@ -152,7 +152,7 @@ def test_c_orthogonalize_refusals(lib):
 
     for dtype in (0, 4):
         refused(call(dtype=dtype), "element type")
-    refused(call(batch=65536), "matrices of")
+    refused(call(batch=32768), "matrices of")
     refused(call(m=-1), "matrices of")
     refused(call(n=(1 << 20) + 1), "matrices of")
     for steps in (0, 65):
