@@ -105,9 +105,11 @@ int lbfgs_train_policy(const lbfgs_train_sequences* seqs, const void* logps, con
 /* the matrix form of an update                                                */
 /* ------------------------------------------------------------------------- */
 /* `batch` dense matrices rows x cols (F32, BF16, F16; batch <= 32767, sides <= 2^20): each is divided by its Frobenius norm (a
- * matrix of zeros stays one), and then `steps` times every singular value s becomes a s + b s^3 + c s^5, the singular vectors
- * staying as they are:  X <- (a I + b S + c S S) X, S = X X^T, in products of 32-bit precision.  Coefficients that lead a
- * singular value of [0, 1] beyond 64, or multiply one by more than 16384 in all, are refused. */
+ * matrix of zeros stays one), and then `steps` times (1 to 64) every singular value s becomes a s + b s^3 + c s^5, the singular
+ * vectors staying as they are:  X <- (a I + b S + c S S) X, S = X X^T.  Products and sums have 32-bit precision or more; for
+ * BF16 and F16 the last steps are taken together, which adds at most 2^-10 (BF16) or 2^-13 (F16) of the result's norm to the
+ * rounding of the result, half of what that alone may be.  Coefficients that lead a singular value of [0, 1] beyond 64, or
+ * multiply one by 128 or more in a step, are refused. */
 uint64_t lbfgs_train_orthogonalize_workspace(int32_t dtype, int64_t batch, int64_t rows, int64_t cols);
 int lbfgs_train_orthogonalize(int32_t dtype, int64_t batch, int64_t rows, int64_t cols, const void* update, void* out, int32_t steps,
                               double a, double b, double c, void* workspace, uint64_t workspace_bytes, void* stream);

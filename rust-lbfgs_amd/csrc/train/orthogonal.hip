@@ -14,12 +14,15 @@
 // Updates of 32 bits go through the steps as written.  Those of 16 bits are exact in hi alone at first (they are scaled by a
 // power of two, the rest of 1/|G| is carried along as a number), and their last few steps work on the Gram matrix: with
 // S = X X^T of the X that they begin with,
-//   P = a I + b S + c S S,   Q <- Q P,   S <- S P P          and in the end   X <- Q X,
+//   P = a I + b S + c S S,   Q <- Q P,   S <- (S P) P        and in the end   X <- Q X,
 // all symmetric and all of the short side, which for a matrix m x 4 m is a third less work.  The price: an error of S is
-// multiplied by up to a^2 in every such step.  Measured with gradients of low rank and noise, 16 x 16 to 400 x 401, five steps in
-// all, against 64 bits and in the Frobenius norm: the last 4 on S add up to 1e-3 to the result (bf16 rounds by 1.7e-3: taken), the
-// last 3 a tenth of that (f16 rounds by 2.1e-4: taken); all 5 would add 2e-3, and in 32 bits not even 2 would do.
-#include "common.h"
+// multiplied by up to a^2 in every such step, and by b where it enters P: of g steps, a rounding of 2^-23 becomes
+// |b| a^(2 g - 2) 2^-23 of the result, which with the usual polynomial is 9.5e-4 for 4 steps and 8e-5 for 3.  So many are taken,
+// of any polynomial, as keep that below 2^-10 for bf16 (which rounds by up to 2^-9) and 2^-13 for f16 (2^-12); in 32 bits not even
+// 2 would do.  Measured against 64 bits with gradients of rank 1, 4 and 32 and noise of 1e-2 to 1e-4, 150 x 200 to 512 x 4000, five
+// steps, in the Frobenius norm: 1.6e-3 to 1.7e-3 for bf16 and 2.1e-4 to 2.2e-4 for f16, which is what rounding the result takes alone;
+// 1.1e-5 to 6.4e-5 for updates of 32 bits.
+#include "orthogonal.h"
 
 #include <algorithm>
 
@@ -64,6 +67,10 @@ struct Halves {
     f16 hi, lo;
 };
 __device__ __forceinline__ Halves split(float v) {
+    // One value for both: a product that v comes from may otherwise be made anew for hi, and rounded to f16 at once there (an
+    // instruction that multiplies and converts), while lo is what is left of its 32-bit rounding: near ties, in one of 2^13
+    // values, the two then are off by a step of hi.
+    asm("" : "+v"(v));
     const f16 hi = (f16)v;
     return {hi, (f16)(v - (float)hi)};
 }
@@ -344,10 +351,22 @@ __global__ __launch_bounds__(WAVES * WAVE, TILE <= 128 && STAGES * TILE <= 256 ?
     asm volatile("" ::: "memory");
     float* const res = (float*)pool;
     auto spot = [](int i, int j) { return j * LINE + (i + 16 * (j >> 3 & 1)) % TILE; };
+    // A symmetric result is exactly so, on the diagonal too: a difference between its halves, as the factors' own roundings make
+    // it where they should commute, grows by more than ten with every step on the Gram matrix (to 8e-3 of a result of bf16).
+    const bool diagonal = (WHAT == SYM || WHAT == POLY) && ti == tj;
 #pragma unroll
     for (int x = 0; x < NI; x++)
 #pragma unroll
-        for (int y = 0; y < NJ; y++) *(float4_*)&res[spot(wi + x * 16 + (lane / 16) * 4, wj + y * 16 + lane % 16)] = PARTS == 3 ? acc[x][y] + low[x][y] : acc[x][y];
+        for (int y = 0; y < NJ; y++) {
+            const float4_ v = PARTS == 3 ? acc[x][y] + low[x][y] : acc[x][y];
+            const int i = wi + x * 16 + (lane / 16) * 4, j = wj + y * 16 + lane % 16;
+            if (!diagonal)
+                *(float4_*)&res[spot(i, j)] = v;
+            else if (wi + x * 16 >= wj + y * 16)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (i + e >= j) res[spot(i + e, j)] = res[spot(j, i + e)] = v[e];
+        }
     __syncthreads();
     float scale = p.scale;
     if (p.inv_power) scale *= p.inv_power == 1 ? p.inv[b] : p.inv[b] * p.inv[b];
@@ -413,8 +432,10 @@ __global__ __launch_bounds__(WAVES * WAVE, TILE <= 128 && STAGES * TILE <= 256 ?
 static int64_t up(int64_t n) { return (n + EDGE - 1) / EDGE * EDGE; }
 
 struct Plan {
-    int m, n, mp, np, batch, steps, gram, tall;  // gram: so many of the steps, the last, work on the Gram matrix
-    double sx, ss, sp, st, sq;  // what X, S, P, P P and Q are multiplied by
+    int m, n, mp, np, batch, steps, tall;
+    int gram;    // so many of the steps, the last, work on the Gram matrix
+    bool brief;  // all of them, in 64 bits (orthogonal_short.hip)
+    double sx, ss, sp, sq;  // what X, S (and S P), P and Q are multiplied by
     double a, b, c;
 };
 struct Buffers {
@@ -450,27 +471,36 @@ static uint64_t lay_out(Buffers* out, void* base, int dtype, int64_t batch, int6
     return at;
 }
 
-// The largest value of X, S, P and Q that singular values in [0, 1] can lead to, and from them the powers of two that keep f16
-// in range.  false: the polynomial leaves it.
-static bool ranges(Plan* q) {
+// How many steps, the last, may work on the Gram matrix: an error of S is multiplied by up to p^2 in each that follows (p: what a
+// step multiplies a singular value by at most) and then by b, and may reach `most`.
+static int gram_steps(const Plan& q, double p, double error, double most) {
+    const double growth = std::max(1.0, p * p);
+    error *= std::max(1.0, std::fabs(q.b));
+    int g = 1;
+    while (g < q.steps && error * growth <= most) error *= growth, g++;
+    return g;
+}
+// The largest values of X, S, P and Q that singular values in [0, 1] can lead to.  From them: how many steps work on the Gram
+// matrix, and the powers of two that keep f16 in range.  false: the polynomial leaves it.
+static bool ranges(Plan* q, int dtype) {
     double x_most = 1.0, p_most = 1.0, q_most = 1.0;
     for (int k = 0; k <= 1000; k++) {
-        double s = k / 1000.0, all = 1.0;
+        double s = k / 1000.0;
         for (int j = 0; j < q->steps; j++) {
             const double l = s * s, p = q->a + q->b * l + q->c * l * l;
             s *= p;
-            if (j >= q->steps - q->gram) all *= p;
             x_most = std::max(x_most, std::fabs(s));
             p_most = std::max(p_most, std::fabs(p));
-            q_most = std::max(q_most, std::fabs(all));
-            if (!(x_most < 64 && p_most < 128 && q_most < 16384)) return false;
+            if (!(x_most < 64 && p_most < 128)) return false;
         }
     }
+    q->brief = q->m <= SHORT && gram_steps(*q, p_most, 0x1p-52, 0x1p-26) == q->steps;
+    q->gram = dtype == LBFGS_TRAIN_F32 ? 0 : gram_steps(*q, p_most, 0x1p-23, dtype == LBFGS_TRAIN_BF16 ? 0x1p-10 : 0x1p-13);
+    for (int j = 0; j < q->gram; j++) q_most *= p_most;  // (2^13.5 at most: p_most^(gram - 1) has passed, < 2^6.5, times 2^7)
     auto scale = [](double most) { return std::exp2(std::floor(std::log2(48000.0 / (most * 1.02)))); };
     q->sx = scale(x_most);
     q->ss = scale(x_most * x_most);
     q->sp = scale(p_most);
-    q->st = scale(p_most * p_most);
     q->sq = scale(q_most);
     return true;
 }
@@ -564,12 +594,12 @@ static void launch_orthogonalize(const Plan& q, const void* g, void* out, const 
         const Split step = k ? f.p : f.q[0];  // (Q = P at first)
         const double step_scale = k ? q.sp : q.sq;
         launch_product<float, POLY, 3>(poly(f.s[now], step, step_scale), nullptr, q.batch, s);
-        Product pp = square(q, step, step, f.t), qp = square(q, f.q[now ^ 1], f.p, f.q[now]);
-        pp.scale = (float)(q.st / (step_scale * step_scale)), qp.scale = (float)(1 / q.sp);
+        Product sp = square(q, f.s[now], step, f.t), qp = square(q, f.q[now ^ 1], f.p, f.q[now]);
+        sp.scale = (float)(1 / step_scale), qp.scale = (float)(1 / q.sp);
         if (more) {
-            launch_product<float, SYM, 3>(pp, k ? &qp : nullptr, q.batch, s);
-            Product next = square(q, f.s[now], f.t, f.s[now ^ 1]);
-            next.scale = (float)(1 / q.st);
+            launch_product<float, SYM, 3>(sp, k ? &qp : nullptr, q.batch, s);
+            Product next = square(q, f.t, step, f.s[now ^ 1]);
+            next.scale = (float)(1 / step_scale);
             launch_product<float, SYM, 3>(next, nullptr, q.batch, s);
         } else if (k) {
             launch_product<float, SYM, 3>(qp, nullptr, q.batch, s);
@@ -588,7 +618,9 @@ using namespace lt;
 
 extern "C" uint64_t lbfgs_train_orthogonalize_workspace(int32_t dtype, int64_t batch, int64_t rows, int64_t cols) {
     if (dtype < LBFGS_TRAIN_F32 || dtype > LBFGS_TRAIN_F16 || batch < 1 || rows < 1 || cols < 1 || batch > 32767 || rows > (1 << 20) || cols > (1 << 20)) return 0;
-    return lay_out(nullptr, nullptr, dtype, batch, rows, cols);
+    const uint64_t size = lay_out(nullptr, nullptr, dtype, batch, rows, cols);
+    const int m = (int)std::min(rows, cols), n = (int)std::max(rows, cols);
+    return m <= SHORT ? std::max(size, short_workspace(batch, m, n)) : size;  // (which of the two it is depends on the steps)
 }
 
 extern "C" int lbfgs_train_orthogonalize(int32_t dtype, int64_t batch, int64_t rows, int64_t cols, const void* update, void* out, int32_t steps, double a, double b,
@@ -600,17 +632,26 @@ extern "C" int lbfgs_train_orthogonalize(int32_t dtype, int64_t batch, int64_t r
         return lt_fail(LBFGS_HIP_ERR_ARG, "%s: %lld matrices of %lld x %lld", who, (long long)batch, (long long)rows, (long long)cols);
     if (steps < 1 || steps > 64) return lt_fail(LBFGS_HIP_ERR_ARG, "%s: %d steps: 1 to 64 are offered", who, steps);
     if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return lt_fail(LBFGS_HIP_ERR_ARG, "%s: coefficients %g, %g, %g", who, a, b, c);
-    Plan q = {(int)std::min(rows, cols), (int)std::max(rows, cols), 0, 0, (int)batch, steps, std::min(steps, dtype == LBFGS_TRAIN_BF16 ? 4 : dtype == LBFGS_TRAIN_F16 ? 3 : 0), rows > cols, 0, 0, 0, 0, 0, a, b, c};
-    if (!ranges(&q)) return lt_fail(LBFGS_HIP_ERR_ARG, "%s: %d steps of %g, %g, %g lead singular values out of range", who, steps, a, b, c);
+    Plan q = {(int)std::min(rows, cols), (int)std::max(rows, cols), 0, 0, (int)batch, steps, rows > cols, 0, false, 0, 0, 0, 0, a, b, c};
+    if (!ranges(&q, dtype)) return lt_fail(LBFGS_HIP_ERR_ARG, "%s: %d steps of %g, %g, %g lead singular values out of range", who, steps, a, b, c);
     if (!batch || !rows || !cols) return LBFGS_HIP_OK;
     if (!update || !out) return lt_fail(LBFGS_HIP_ERR_ARG, "%s: update and out are needed", who);
     q.mp = (int)up(q.m), q.np = (int)up(q.n);
-    const uint64_t need = lay_out(nullptr, nullptr, dtype, batch, rows, cols);
+    const uint64_t need = lbfgs_train_orthogonalize_workspace(dtype, batch, rows, cols);
     if (!workspace || workspace_bytes < need)
         return lt_fail(LBFGS_HIP_ERR_ARG, "%s: %llu bytes of workspace, %llu are needed", who, (unsigned long long)(workspace ? workspace_bytes : 0), (unsigned long long)need);
+    hipStream_t s = (hipStream_t)stream;
+    if (q.brief) {
+        const Short p = {update, out, workspace, q.m, q.n, q.tall, q.batch, q.steps, a, b, c};
+        switch (dtype) {
+            case LBFGS_TRAIN_F32: short_orthogonalize<float>(p, s); break;
+            case LBFGS_TRAIN_BF16: short_orthogonalize<bf16>(p, s); break;
+            default: short_orthogonalize<f16>(p, s);
+        }
+        return lt_launched(who);
+    }
     Buffers f;
     lay_out(&f, workspace, dtype, batch, rows, cols);
-    hipStream_t s = (hipStream_t)stream;
     switch (dtype) {
         case LBFGS_TRAIN_F32: launch_orthogonalize<float>(q, update, out, f, s); break;
         case LBFGS_TRAIN_BF16: launch_orthogonalize<bf16>(q, update, out, f, s); break;
