@@ -54,7 +54,7 @@ typedef struct lbfgs_train_rows {
 /*   logps[t] = (x_t[y_t] - m_t)/temperature - l_t,   m_t = max_v x_t[v],   l_t = log sum_v exp((x_t[v] - m_t)/temperature)
  * logps in the wide type; lse[2 t] = m_t and lse[2 t + 1] = l_t in 64 bits, the log-sum-exp in two parts: their sum would lose
  * the second where the first is large, as in a row masked by its type's lowest value.
- * A target outside [0, vocab) that is not ignore_index gives NaN. */
+ * A target outside [0, vocab) that is not ignore_index gives NaN.  Temperatures: 1e-37 to 1e37, for F64 1e-300 to 1e300. */
 uint64_t lbfgs_train_token_logprobs_workspace(int32_t dtype, int64_t rows, int64_t vocab);
 int lbfgs_train_token_logprobs(const lbfgs_train_rows* rows, double temperature, void* logps, double* lse, void* workspace,
                                uint64_t workspace_bytes, void* stream);

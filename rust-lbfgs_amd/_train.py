@@ -87,6 +87,8 @@ def floating(name, t):
         raise TypeError(f"{name} must be a torch tensor, not {type(t).__name__}")
     if t.dtype not in DTYPES:
         raise TypeError(f"{name} must be float64, float32, bfloat16 or float16, not {t.dtype}")
+    if t.is_neg():
+        raise TypeError(f"{name} is a view whose sign is still to be applied: resolve_neg() first")
 
 
 def on_gpu(name, t, others=()):
@@ -106,6 +108,8 @@ def like(name, t, what, dtype, shape):
         raise TypeError(f"{name} must be a torch tensor, not {type(t).__name__}")
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype} as {what} asks for, not {t.dtype}")
+    if t.is_neg():
+        raise TypeError(f"{name} is a view whose sign is still to be applied: resolve_neg() first")
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)} as {what} asks for, not {tuple(t.shape)}")
 
@@ -126,7 +130,7 @@ def enqueue(function, device, *arguments):
 
 
 def refuse_capture(what, instead):
-    """Autograd inside a stream capture goes through the leaf's accumulation node, and where an eager graph of the same leaf
-    keeps that node alive on another stream, torch ends the process.  The call cannot see that, so it is refused."""
+    """Autograd inside a stream capture goes through the leaf's accumulation node, and where an eager graph of the same leaf keeps
+    that node alive on another stream, torch ends the process.  The call cannot see that, so it is refused."""
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError(f"{what} with a gradient to come cannot be captured into a graph: capture {instead}, which need no autograd")

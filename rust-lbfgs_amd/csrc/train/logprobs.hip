@@ -296,6 +296,9 @@ static int check_rows(const lbfgs_train_rows* q, double temperature, Rows* r, co
         (q->inner && q->outer > (INT64_MAX >> 20) / q->inner))
         return lt_fail(LBFGS_HIP_ERR_ARG, "%s: %lld x %lld rows of %lld logits", who, (long long)q->outer, (long long)q->inner, (long long)q->vocab);
     if (!(temperature > 0) || !std::isfinite(temperature)) return lt_fail(LBFGS_HIP_ERR_ARG, "%s: temperature %g is not a positive number", who, temperature);
+    if (q->dtype != LBFGS_TRAIN_F64 && !(temperature >= 1e-37 && temperature <= 1e37))  // (its reciprocal is a number of 32 bits)
+        return lt_fail(LBFGS_HIP_ERR_ARG, "%s: temperature %g is out of range: 1e-37 to 1e37 for this element type", who, temperature);
+    if (!(temperature >= 1e-300 && temperature <= 1e300)) return lt_fail(LBFGS_HIP_ERR_ARG, "%s: temperature %g is out of range: 1e-300 to 1e300", who, temperature);
     *r = {q->outer * q->inner, q->inner, q->outer_stride, q->inner_stride, q->vocab, q->targets, q->ignore_index};
     if (r->rows && (!q->logits || !q->targets)) return lt_fail(LBFGS_HIP_ERR_ARG, "%s: logits and targets are needed", who);
     return LBFGS_HIP_OK;

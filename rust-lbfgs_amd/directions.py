@@ -23,6 +23,7 @@ def orthogonalize(update, *, steps=5, coefficients=COEFFICIENTS):
     Products have 32-bit precision or more for all types, and the result is rounded once; for 16-bit types the last steps are
     taken together, which adds at most half of that rounding's bound (2^-10 of the result's norm in bfloat16, 2^-13 in float16).
     Coefficients that lead singular values of [0, 1] beyond 64, or multiply one by 128 or more in a step, are refused.
+    A direction, not a part of the loss: nothing is recorded for autograd.
     A matrix that holds a NaN or an infinity gives NaN, the others of its batch are not touched by it."""
     _train.floating("update", update)
     if update.dtype == torch.float64:

@@ -101,6 +101,7 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
+        _train.refuse_capture("the backward pass of token_logprobs", "token_logprobs_grad")
         logits, targets, lse = ctx.saved_tensors
         return token_logprobs_grad(logits, targets, lse, grad, *ctx.extra), None, None, None
 
@@ -216,7 +217,11 @@ class _ValueAndGrad(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, up):
-        return ctx.saved_tensors[0] * up.to(ctx.saved_tensors[0].dtype), None
+        _train.refuse_capture("the backward pass of a loss", "preference or policy")
+        (grad,) = ctx.saved_tensors
+        if grad.dtype == up.dtype:
+            return grad * up, None
+        return (grad.to(up.dtype) * up).to(grad.dtype), None  # (16 bits: what comes in is not rounded, the product is)
 
 
 def _differentiable(name, logps, result):

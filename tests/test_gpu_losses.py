@@ -106,6 +106,34 @@ def test_logprobs_temperature(tau):
         check_logprobs(*make((9,), 515, dtype), tau)
 
 
+@pytest.mark.parametrize("dtype, taus", [("f32", (1e-37, 1e37)), ("bf16", (1e-37, 1e37)), ("f64", (1e-300, 1e300))])
+def test_logprobs_extreme_temperatures(dtype, taus):
+    """All the weight on the largest logit, or the same for each that is not masked; a gradient's factor 1/temperature in the upstream one."""
+    x = torch.arange(16, device="cuda").to(DT[dtype])
+    x[::4] = -math.inf
+    y = torch.tensor([15], device="cuda")
+    for tau, want in zip(taus, (0.0, -math.log(12))):
+        lp, lse = losses.token_logprobs_with_lse(x[None], y, tau)
+        assert abs(float(lp) - want) <= 4e-7  # a logarithm and a sum of 12 ones in 32 bits
+        d = losses.token_logprobs_grad(x[None], y, lse, torch.full_like(lp, tau), tau).double()[0]
+        p = torch.zeros(16, dtype=torch.float64, device="cuda")
+        p[15 if want == 0 else slice(None)] = 1 if want == 0 else 1 / 12
+        p[::4] = 0
+        onehot = torch.nn.functional.one_hot(y[0], 16)
+        # tau/tau through 32 bits, an exponential, the rounding of the result
+        assert ((d - (onehot - p)).abs() <= 1e-6 + torch.finfo(x.dtype).eps / 2).all(), tau
+
+
+def test_what_comes_into_a_loss_is_not_rounded_to_16_bits():
+    for dtype in (torch.bfloat16, torch.float16):
+        x = torch.randn(4, 700, generator=torch.Generator().manual_seed(0)).cuda().to(dtype).requires_grad_()
+        up = torch.tensor(1 / 3, device="cuda")
+        losses.preference_loss(x).backward(up)
+        want = losses.preference(x.detach()).grad.double() * up.double()
+        # the product in 32 bits, rounded once more
+        assert ((x.grad.double() - want).abs() <= want.abs() * (torch.finfo(dtype).eps / 2 + 2.0 ** -23) + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2).all()
+
+
 @pytest.mark.parametrize("dtype", DT)
 def test_logprobs_ignored_and_out_of_range_targets(dtype):
     x, y, g = make((12,), 999, DT[dtype])

@@ -93,6 +93,10 @@ def test_c_logprobs_refusals(lib):
     for t in (0.0, -1.0, math.nan, math.inf):
         refused(lib.lbfgs_train_token_logprobs(rows(), t, P, P, P, 1 << 30, None), "temperature")
         refused(lib.lbfgs_train_token_logprobs_grad(rows(), t, P, P, P, None), "temperature")
+    for dtype, values in ((0, (1e-301, 1e301)), (1, (1e-38, 1e38)), (2, (1e-38, 1e38)), (3, (1e-38, 1e38))):
+        for t in values:
+            refused(lib.lbfgs_train_token_logprobs(rows(dtype=dtype), t, P, P, P, 1 << 30, None), "out of range")
+            refused(lib.lbfgs_train_token_logprobs_grad(rows(dtype=dtype), t, P, P, P, None), "out of range")
     refused(lib.lbfgs_train_token_logprobs(None, 1.0, P, P, P, 0, None), "no rows")
     refused(lib.lbfgs_train_token_logprobs(rows(), 1.0, None, P, P, 0, None), "are needed")
     refused(lib.lbfgs_train_token_logprobs(rows(), 1.0, P, None, P, 0, None), "are needed")
@@ -238,6 +242,16 @@ def test_orthogonalize_refusals(lib):
         directions.orthogonalize(torch.zeros(3))
     with pytest.raises(ValueError, match="coefficients"):
         directions.orthogonalize(torch.zeros(2, 3), coefficients=(1.0, 2.0))
+
+
+def test_views_with_a_sign_to_come_are_refused(lib):
+    lazy = torch.view_as_complex(torch.ones(6, 2)).conj().imag
+    assert lazy.is_neg()
+    off = torch.tensor([0, 2, 6])
+    for call in (lambda: losses.token_logprobs(lazy, torch.tensor(0)), lambda: losses.preference(lazy, offsets=off), lambda: losses.preference(torch.ones(6), lazy, offsets=off),
+                 lambda: losses.policy(torch.ones(6), torch.ones(6), lazy, offsets=off), lambda: directions.orthogonalize(lazy.view(2, 3))):
+        with pytest.raises(TypeError, match="resolve_neg"):
+            call()
 
 
 def test_modules_are_reached_from_the_package():
