@@ -36,11 +36,11 @@ def orthogonalize(update, *, steps=5, coefficients=COEFFICIENTS):
     dev = _train.on_gpu("update", update)
     L = _train.load()
     g = update if update.is_contiguous() else update.detach().contiguous()
-    out = torch.empty(g.shape, dtype=g.dtype, device=dev)
+    out = g.new_empty(g.shape)
     rows, cols = g.shape[-2:]
     batch = g.numel() // (rows * cols) if rows and cols else 0
     size = L.lbfgs_train_orthogonalize_workspace(_train.DTYPES[g.dtype], batch, rows, cols)
-    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    ws = g.new_empty(size, dtype=torch.uint8) if size else None
     _train.enqueue(L.lbfgs_train_orthogonalize, dev, _train.DTYPES[g.dtype], batch, rows, cols, g.data_ptr(), out.data_ptr(), steps, *coefficients,
                    _train.ptr(ws), size)
     return out

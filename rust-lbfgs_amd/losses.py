@@ -64,10 +64,10 @@ def token_logprobs_with_lse(logits, targets, temperature=1.0, ignore_index=-100)
     row is not read; any other target outside [0, V) gives NaN.  Masked logits may be -inf or the type's lowest value."""
     rows, dev, keep = _rows(logits, targets, ignore_index)
     L = _train.load()
-    logps = torch.empty(targets.shape, dtype=_train.wide(logits.dtype), device=dev)
-    lse = torch.empty((*targets.shape, 2), dtype=torch.float64, device=dev)
+    logps = logits.new_empty(targets.shape, dtype=_train.wide(logits.dtype))
+    lse = logits.new_empty((*targets.shape, 2), dtype=torch.float64)
     size = L.lbfgs_train_token_logprobs_workspace(rows.dtype, rows.outer * rows.inner, rows.vocab)
-    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    ws = logits.new_empty(size, dtype=torch.uint8) if size else None
     _train.enqueue(L.lbfgs_train_token_logprobs, dev, C.byref(rows), temperature, logps.data_ptr(), lse.data_ptr(), _train.ptr(ws), size)
     del keep
     return logps, lse
@@ -84,7 +84,7 @@ def token_logprobs_grad(logits, targets, lse, grad, temperature=1.0, ignore_inde
     _train.on_gpu("logits", logits, (("lse", lse), ("grad", grad)))
     L = _train.load()
     lse, grad = lse.contiguous(), grad.contiguous()
-    out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    out = logits.new_empty(logits.shape)
     _train.enqueue(L.lbfgs_train_token_logprobs_grad, dev, C.byref(rows), temperature, lse.data_ptr(), grad.data_ptr(), out.data_ptr())
     del keep
     return out
@@ -166,10 +166,10 @@ def preference(logps, ref_logps=None, *, offsets=None, mask=None, beta=0.1, kind
     q, count, (x, m, o, ref) = _sequences(logps, offsets, mask, others)
     dev = _train.on_gpu("logps", logps, (("offsets", offsets), ("mask", mask), *others))
     L, out = _train.load(), _train.wide(x.dtype)
-    f, rewards = torch.empty((), dtype=out, device=dev), torch.empty(count, dtype=out, device=dev)
-    grad = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    f, rewards = x.new_empty((), dtype=out), x.new_empty(count, dtype=out)
+    grad = torch.empty_like(x)
     size = L.lbfgs_train_sequences_workspace(q.tokens, count)
-    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    ws = x.new_empty(size, dtype=torch.uint8) if size else None
     _train.enqueue(L.lbfgs_train_preference, dev, C.byref(q), x.data_ptr(), _train.ptr(ref), beta, label_smoothing, KINDS[kind], bool(normalize_lengths),
                    f.data_ptr(), rewards.data_ptr(), grad.data_ptr(), _train.ptr(ws), size)
     return Preference(f, rewards, grad)
@@ -199,10 +199,10 @@ def policy(logps, old_logps, advantages, *, ref_logps=None, offsets=None, mask=N
     _train.like("advantages", advantages, "logps (or [sequences, 1])", x.dtype, x.shape if per_token else (count, 1))
     dev = _train.on_gpu("logps", logps, (("offsets", offsets), ("mask", mask), ("advantages", advantages), *others))
     L, adv = _train.load(), _dense(advantages)
-    f, kl, clipped = torch.empty(3, dtype=_train.wide(x.dtype), device=dev).unbind()
-    grad = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    f, kl, clipped = x.new_empty(3, dtype=_train.wide(x.dtype)).unbind()
+    grad = torch.empty_like(x)
     size = L.lbfgs_train_sequences_workspace(q.tokens, count)
-    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    ws = x.new_empty(size, dtype=torch.uint8) if size else None
     _train.enqueue(L.lbfgs_train_policy, dev, C.byref(q), x.data_ptr(), old.data_ptr(), _train.ptr(ref), adv.data_ptr(), per_token, clip_low, clip_high, kl_coef,
                    REDUCTIONS[reduction], f.data_ptr(), kl.data_ptr(), clipped.data_ptr(), grad.data_ptr(), _train.ptr(ws), size)
     return Policy(f, kl, clipped, grad)
