@@ -234,11 +234,14 @@ constexpr int64_t MOST_BLOCKS = 1 << 22;  // a launch has less than 2^32 threads
 
 static int64_t elem_size(int dtype) { return dtype == LBFGS_TRAIN_F64 ? 8 : dtype == LBFGS_TRAIN_F32 ? 4 : 2; }
 
-// workgroups to a row of the forward pass
+// Workgroups to a row of the forward pass: several, with a second launch to join them, only where few rows are long enough for one
+// workgroup to need some 10 us more than that launch.  Measured for 1 and 64 rows, shared and not, in us: 131072 in f64 8.5 and 21
+// (39, 47), 131072 in f32 8.1 and 9.4 (9.8, 11.1) and in bf16 8.3 and 8.9 (8.9, 10.5), 32768 in bf16 7.6 and 8.0 (4.1, 5.1).  A
+// launch takes 3 us of the host beside.
 static int forward_splits(int64_t rows, int64_t vocab, int dtype) {
-    const int64_t bytes = vocab * elem_size(dtype);
-    if (rows >= 256 || bytes < 65536) return 1;
-    const int64_t want = (512 + rows - 1) / rows, most = bytes / 16384;
+    const int64_t cost = vocab * (dtype == LBFGS_TRAIN_F64 ? 6 : 1);  // (exponentials of 64 bits)
+    if (rows > 128 || cost < 196608) return 1;
+    const int64_t want = (512 + rows - 1) / rows, most = vocab * elem_size(dtype) / 16384;
     return (int)(want < most ? want : most);
 }
 static int64_t part_of(int64_t vocab, int splits) {
@@ -259,13 +262,18 @@ static void launch_forward(const void* x, const Rows& r, double tau, void* logps
         MaxSum<A>* found = (MaxSum<A>*)ws;
         logprobs_part_kernel<T, 256><<<dim3(splits, (unsigned)r.rows), 256, 0, s>>>((const T*)x, r, c, part, found);
         logprobs_join_kernel<T><<<(unsigned)r.rows, WAVE, 0, s>>>((const T*)x, r, tau, c, splits, found, (A*)logps, lse);
-    } else if (bytes <= 4096) {
-        logprobs_kernel<T, 64><<<(unsigned)grid, 64, 0, s>>>((const T*)x, r, tau, c, (A*)logps, lse);
-    } else if (bytes <= 131072) {  // (a row of 64 KiB: 112 us for 8192 of them with 128, 256 or 512 threads, 148 with 1024)
-        logprobs_kernel<T, 256><<<(unsigned)grid, 256, 0, s>>>((const T*)x, r, tau, c, (A*)logps, lse);
-    } else {  // (256 KiB: 351 us with 256, 346 with 512, 354 with 1024)
-        logprobs_kernel<T, 512><<<(unsigned)grid, 512, 0, s>>>((const T*)x, r, tau, c, (A*)logps, lse);
+        return;
     }
+    // Many rows fill the chip with a wave each, few need the whole workgroup.  Measured in bf16 with 64, 256 and 512 threads, in us:
+    // 4000 rows of 4000 10.4, 12.2, 19.0, of 8192 14.3, 15.9, 22.7, of 16384 23.6, 24.1, 28.8, of 32768 42.2, 41.3, 41.6, of 131072 184, 179,
+    // 175; 64 rows of 1000 3.5, 3.6, 3.7, of 4000 4.5, 3.8, 3.7, of 16384 6.9, 4.4, 4.3, of 32768 10.5, 5.4, 5.1, of 131072 34, 11.2, 10.5.
+    const bool many = r.rows >= 1024;
+    if (bytes <= (many ? 16384 : 4096))
+        logprobs_kernel<T, 64><<<(unsigned)grid, 64, 0, s>>>((const T*)x, r, tau, c, (A*)logps, lse);
+    else if (bytes <= (many ? 131072 : 32768))
+        logprobs_kernel<T, 256><<<(unsigned)grid, 256, 0, s>>>((const T*)x, r, tau, c, (A*)logps, lse);
+    else
+        logprobs_kernel<T, 512><<<(unsigned)grid, 512, 0, s>>>((const T*)x, r, tau, c, (A*)logps, lse);
 }
 
 template <class T>
@@ -273,12 +281,12 @@ static void launch_grad(const void* x, const Rows& r, double tau, const double* 
     typedef typename Num<T>::acc A;
     const A c = (A)(1.4426950408889634 / tau);
     const int64_t bytes = r.vocab * (int64_t)sizeof(T);
-    int64_t splits = 1;
-    if (r.rows < 2048) {
-        splits = (2048 + r.rows - 1) / r.rows;
-        const int64_t most = (bytes + 8191) / 8192;
-        if (splits > most) splits = most;
-    }
+    // Workgroups to a row: so many that there are 512, of 16 KiB at least.  Measured in bf16 for one to a row, 512 and 2048 in all, in us:
+    // 64 rows of 131072 16.6, 6.7, 9.8, 1 row 14.5, 3.2, 3.3, 255 rows of 32768 9.3, 6.9, 9.8, 1000 of 8192 6.9, 6.9, 9.8.
+    const int64_t most = bytes / 16384;
+    int64_t splits = 512 / r.rows;
+    splits = splits < most ? splits : most;
+    if (splits < 1) splits = 1;
     const int64_t part = part_of(r.vocab, (int)splits);
     splits = (r.vocab + part - 1) / part;
     const int64_t units = r.rows * splits;

@@ -258,6 +258,8 @@ __global__ __launch_bounds__(256) void short_apply_kernel(const T* g, int m, int
 }
 
 // Slices: a chunk of 64 columns takes some 1.5 us of a workgroup, adding up a slice 0.2 us; and no more than the device has use for.
+// Measured, the three kernels at 64 x n, in us, with 8, 32 and 79 slices and with the rule's: n = 1000 51, 50, 50, 52; 5000 72, 59, 67, 60;
+// 100000 747, 252, 165, 155.
 static int slices_of(int64_t batch, int n) {
     const double chunks = (n + 63) / 64;
     return (int)std::max(1.0, std::min({chunks, std::sqrt(7.5 * chunks), 256.0, std::ceil(1024.0 / batch)}));

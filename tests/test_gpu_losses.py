@@ -100,6 +100,19 @@ def test_logprobs_row_shared_by_workgroups(V):
     check_logprobs(*make((1,), V, torch.float64), 1.0)
 
 
+@pytest.mark.parametrize("dtype, V", [("bf16", 200003), ("f32", 262147), ("f64", 40001), ("f16", 196609)])
+def test_logprobs_long_row_shared_by_workgroups(dtype, V):
+    for rows in (1, 2, 128, 129):
+        check_logprobs(*make((rows,), V, DT[dtype], sharp=5.0), 1.3)
+
+
+@pytest.mark.parametrize("V", [2047, 2049, 8191, 8193, 16385, 65537])
+def test_logprobs_workgroups_of_every_size(V):
+    """Waves, workgroups of four and of eight for a row, with few rows and many; rows of the gradient whole and shared."""
+    for rows in (1, 100, 300, 1024):
+        check_logprobs(*make((rows,), V, torch.bfloat16, sharp=5.0), 0.9)
+
+
 @pytest.mark.parametrize("tau", [1e-2, 0.5, 3.0, 100.0])
 def test_logprobs_temperature(tau):
     for dtype in DT.values():

@@ -101,10 +101,10 @@ def test_c_logprobs_refusals(lib):
     refused(lib.lbfgs_train_token_logprobs(rows(), 1.0, None, P, P, 0, None), "are needed")
     refused(lib.lbfgs_train_token_logprobs(rows(), 1.0, P, None, P, 0, None), "are needed")
     refused(lib.lbfgs_train_token_logprobs_grad(rows(), 1.0, P, P, None, None), "are needed")
-    need = lib.lbfgs_train_token_logprobs_workspace(2, 2, 100000)
-    assert need > 0 and lib.lbfgs_train_token_logprobs_workspace(2, 100000, 100000) == 0
-    refused(lib.lbfgs_train_token_logprobs(rows(dtype=2, vocab=100000), 1.0, P, P, P, need - 1, None), "workspace")
-    refused(lib.lbfgs_train_token_logprobs(rows(dtype=2, vocab=100000), 1.0, P, P, None, need, None), "workspace")
+    need = lib.lbfgs_train_token_logprobs_workspace(2, 2, 400000)
+    assert need > 0 and lib.lbfgs_train_token_logprobs_workspace(2, 100000, 400000) == 0
+    refused(lib.lbfgs_train_token_logprobs(rows(dtype=2, vocab=400000), 1.0, P, P, P, need - 1, None), "workspace")
+    refused(lib.lbfgs_train_token_logprobs(rows(dtype=2, vocab=400000), 1.0, P, P, None, need, None), "workspace")
     assert lib.lbfgs_train_token_logprobs(rows(outer=0), 1.0, None, None, None, 0, None) == 0  # no rows: nothing to do
 
 
