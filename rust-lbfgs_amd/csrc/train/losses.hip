@@ -424,6 +424,7 @@ __global__ __launch_bounds__(BLOCK) void slopes_kernel(Seqs q, int64_t chunks, i
 // Not too many pairs: no pass of their own (in us, without and with: 512 sequences of 200 10.2, 13.4; 2048 of 512 16.0, 13.4).  A chunk's workgroup finds the slopes of its sequences itself, from their sums and
 // their partners'; the last workgroup, which has no chunk, the loss and the rewards.
 constexpr int64_t FEW_SEQS = 1024;  // (a power of two)
+constexpr int64_t FEW_LONG_SEQS = 128;  // ... of many chunks (in us: 128 of 20000 16.9, 17.9; 256 of 20000 27.6, 24.9; 1000 of 8200 63, 32)
 template <class T, int GROUP>
 __global__ __launch_bounds__(BLOCK) void few_slopes_kernel(Seqs q, Preference o, int64_t chunks, Space sp, typename Num<T>::acc* f, typename Num<T>::acc* rewards, T* grad) {
     __shared__ double slope[FEW_SEQS];
@@ -841,7 +842,7 @@ static void launch_preference(const Seqs& q, const Preference& o, const void* a,
     const int blocks = (int)(groups < LOSS_BLOCKS ? groups : LOSS_BLOCKS);
     const unsigned grid = (unsigned)(chunks < (1 << 20) ? (chunks ? chunks : 1) : (1 << 20));
     if (chunks) sums_kernel<T><<<grid, BLOCK, 0, s>>>(q, (const T*)a, (const T*)b, chunks, sp);
-    if (q.count <= FEW_SEQS) {
+    if (q.count <= (many ? FEW_LONG_SEQS : FEW_SEQS)) {
         const unsigned grid = (unsigned)(chunks < 768 ? chunks : 768);  // (three to a compute unit: all of them at once)
         if (many)
             few_slopes_kernel<T, 8><<<grid + 1, BLOCK, 0, s>>>(q, o, chunks, sp, (A*)f, (A*)rewards, (T*)grad);

@@ -334,6 +334,13 @@ def test_preference(lengths, layout, dtype):
         assert (got.grad.reshape(-1).cpu()[~keep] == 0).all()
 
 
+@pytest.mark.parametrize("count", [64, 128, 130])
+def test_preference_of_many_long_sequences(count, monkeypatch):
+    """More than four chunks each: their records are added up by groups of lanes, where slopes are wanted or in a pass of its own."""
+    monkeypatch.setitem(LENGTHS, "many long", [8250 + 13 * (k % 17) for k in range(count)])
+    test_preference("many long", "packed", "f32")
+
+
 def test_preference_extreme_margins():
     """Margins far beyond where exp overflows, and an infinite one."""
     lp = torch.tensor([[0.0], [-2e4], [-1e30], [-math.inf], [-2e4], [0.0], [0.0], [0.0]], dtype=torch.float64).cuda()
