@@ -3,7 +3,9 @@
 //   l_t  = x_t[y_t]/tau - log sum_v exp(x_tv/tau)            dx_tv = g_t/tau * (1[v = y_t] - exp(x_tv/tau - lse_t))
 //
 // Both are bound by HBM: the forward pass reads every logit once (running maximum and sum in registers), the gradient
-// reads it once more and writes as much.
+// reads it once more and writes as much.  Measured in bf16 (a copy of 2 GiB: 4.93 TB/s, read and written): 8192 x 131072 forward
+// 347 us, 6.2 TB/s; 8192 x 32768 forward 111 us, 4.8 TB/s, gradient 176 us, 6.1 TB/s, part of what it reads being in the caches yet;
+// rows of odd length in 32 bits, 16-byte loads at any alignment, 5.2 TB/s.  Few rows are bound by the launch: 8 rows of 32768 5 us.
 #include "common.h"
 
 namespace lt {

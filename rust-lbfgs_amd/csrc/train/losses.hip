@@ -8,6 +8,10 @@
 //     tail[w]   for the one that starts in chunk w and goes on,       head[w]  for the one that started before chunk w,
 // and whoever needs a sequence's sum adds tail + heads + head in chunk order: no atomics, one order, the same bits always.
 // Every sum over tokens is held in 64 bits: the values wanted are differences of sums of thousands of terms.
+//
+// Large batches are bound by HBM, all others by launches and by how few loads wait for each other.  Measured in 32 bits: policy,
+// 8.4 million tokens, a reference and a mask: 7 us to count, 32 for losses and gradients (5.5 TB/s), 5 for the results; preference,
+// 48 sequences of up to 131072 tokens: sums 8 us (3.7 TB/s), slopes, loss and gradient 15; 512 of up to 2047: 5 and 6 us.
 #include "common.h"
 
 namespace lt {
