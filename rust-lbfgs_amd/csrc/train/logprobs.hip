@@ -8,6 +8,8 @@
 // rows of odd length in 32 bits, 16-byte loads at any alignment, 5.2 TB/s.  Few rows are bound by the launch: 8 rows of 32768 5 us.
 #include "common.h"
 
+#include <algorithm>
+
 namespace lt {
 
 template <class A>
@@ -283,12 +285,11 @@ static void launch_grad(const void* x, const Rows& r, double tau, const double* 
     typedef typename Num<T>::acc A;
     const A c = (A)(1.4426950408889634 / tau);
     const int64_t bytes = r.vocab * (int64_t)sizeof(T);
-    // Workgroups to a row: so many that there are 512, of 16 KiB at least.  Measured in bf16 for one to a row, 512 and 2048 in all, in us:
-    // 64 rows of 131072 16.6, 6.7, 9.8, 1 row 14.5, 3.2, 3.3, 255 rows of 32768 9.3, 6.9, 9.8, 1000 of 8192 6.9, 6.9, 9.8.
-    const int64_t most = bytes / 16384;
-    int64_t splits = 512 / r.rows;
-    splits = splits < most ? splits : most;
-    if (splits < 1) splits = 1;
+    // Workgroups to a row: so many that there are 512 of 16 KiB at least, or 2048 of 64 KiB.  Measured for one to a row, 512 and 2048 in all,
+    // in us: in bf16 64 rows of 131072 16.6, 6.7, 9.8, 1 row 14.5, 3.2, 3.3, 255 rows of 32768 9.3, 6.9, 9.8, 1000 of 8192 6.9, 6.9, 9.8; in
+    // f32, forward and gradient, 1020 of 50001 123, 123, 117.
+    auto shares = [&](int64_t all, int64_t least) { return std::min(all / r.rows, bytes / least); };
+    int64_t splits = std::max<int64_t>({1, shares(512, 16384), shares(2048, 65536)});
     const int64_t part = part_of(r.vocab, (int)splits);
     splits = (r.vocab + part - 1) / part;
     const int64_t units = r.rows * splits;
