@@ -37,7 +37,7 @@ HIP_SRCS = HIP_UNITS + [os.path.join(CSRC, f) for f in ("ctx.h", "ops.h", "strea
 SOLVER_SRCS = [os.path.join(CSRC, "host", "solver.cpp"), os.path.join(ROOT, "include", "lbfgs_solver.h"),
                os.path.join(ROOT, "include", "lbfgs_hip.h")]
 
-TRAIN_UNITS = [os.path.join(CSRC, "train", f) for f in ("losses.hip", "logprobs.hip", "orthogonal.hip", "orthogonal_short.hip")]
+TRAIN_UNITS = [os.path.join(CSRC, "train", f) for f in ("losses.hip", "logprobs.hip", "orthogonal.hip", "orthogonal_short.hip", "orthogonal_panel.hip")]
 TRAIN_SRCS = TRAIN_UNITS + [os.path.join(CSRC, "train", "common.h"), os.path.join(CSRC, "train", "orthogonal.h"), os.path.join(ROOT, "include", "lbfgs_train.h"),
                             os.path.join(ROOT, "include", "lbfgs_hip.h")]
 

@@ -28,14 +28,8 @@
 
 namespace lt {
 
-typedef f16 half8 __attribute__((ext_vector_type(8)));
-typedef f16 half2 __attribute__((ext_vector_type(2)));
-typedef f16 half4 __attribute__((ext_vector_type(4)));
-typedef float float4_ __attribute__((ext_vector_type(4)));
-
 constexpr int EDGE = 64;     // sides are padded to multiples of it, with zeros ...
 constexpr int SPARE = 256;  // ... and so many rows behind a matrix are memory, with whatever they hold: tiles reach beyond the last row
-constexpr int NORM_BLOCKS = 256;
 
 struct Split {  // hi and lo parts, dense, padded with zeros to multiples of EDGE
     f16 *hi, *lo;
@@ -68,19 +62,6 @@ __global__ __launch_bounds__(256) void norm_kernel(const T* g, int64_t n, double
     if (threadIdx.x % WAVE == 0) w[threadIdx.x / WAVE] = s;
     __syncthreads();
     if (threadIdx.x == 0) part[blockIdx.y * NORM_BLOCKS + blockIdx.x] = w[0] + w[1] + w[2] + w[3];
-}
-
-// (by value: halves of a vector are no lvalues to refer to)
-struct Halves {
-    f16 hi, lo;
-};
-__device__ __forceinline__ Halves split(float v) {
-    // One value for both: a product that v comes from may otherwise be made anew for hi, and rounded to f16 at once there (an
-    // instruction that multiplies and converts), while lo is what is left of its 32-bit rounding: near ties, in one of 2^13
-    // values, the two then are off by a step of hi.
-    asm("" : "+v"(v));
-    const f16 hi = (f16)v;
-    return {hi, (f16)(v - (float)hi)};
 }
 
 // X (m x n, K = n adjacent) and its transpose from G or, tall, from G^T: X = G * factor, and *inv what X has to be multiplied by
@@ -552,12 +533,23 @@ static Product square(const Plan& q, Split l, Split r, Split o) {
     return p;
 }
 
+static int norm_blocks(const Plan& q) { return (int)std::min<int64_t>(NORM_BLOCKS, ((int64_t)q.m * q.n + 4095) / 4096); }
+template <class T>
+static void launch_norm(const Plan& q, const void* g, double* part, hipStream_t s) {
+    norm_kernel<T><<<dim3(norm_blocks(q), q.batch), 256, 0, s>>>((const T*)g, (int64_t)q.m * q.n, part);
+}
+template <class T>
+static void launch_panels(const Plan& q, const Panel& p, hipStream_t s) {
+    launch_norm<T>(q, p.update, (double*)p.workspace, s);
+    panel_orthogonalize<T>(p, s);
+}
+
 template <class T>
 static void launch_orthogonalize(const Plan& q, const void* g, void* out, const Buffers& f, hipStream_t s) {
     constexpr bool WHOLE = sizeof(T) == 2;
-    const int64_t size = (int64_t)q.m * q.n, X = (int64_t)q.mp * q.np;
-    const int blocks = (int)std::min<int64_t>(NORM_BLOCKS, (size + 4095) / 4096);
-    norm_kernel<T><<<dim3(blocks, q.batch), 256, 0, s>>>((const T*)g, size, f.part);
+    const int64_t X = (int64_t)q.mp * q.np;
+    const int blocks = norm_blocks(q);
+    launch_norm<T>(q, g, f.part, s);
     split_kernel<T><<<dim3(q.np / 64, q.mp / 64, q.batch), 256, 0, s>>>((const T*)g, q.m, q.n, q.mp, q.np, q.tall, f.part, blocks, q.sx, f.x[0], f.xt[0], f.inv);
     auto gram = [&](int at) {  // S = X X^T
         Product p = square(q, f.x[at], f.x[at], f.s[0]);
@@ -632,7 +624,8 @@ extern "C" uint64_t lbfgs_train_orthogonalize_workspace(int32_t dtype, int64_t b
     if (dtype < LBFGS_TRAIN_F32 || dtype > LBFGS_TRAIN_F16 || batch < 1 || rows < 1 || cols < 1 || batch > 32767 || rows > (1 << 20) || cols > (1 << 20)) return 0;
     const uint64_t size = lay_out(nullptr, nullptr, dtype, batch, rows, cols);
     const int m = (int)std::min(rows, cols), n = (int)std::max(rows, cols);
-    return m <= SHORT ? std::max(size, short_workspace(batch, m, n)) : size;  // (which of the two it is depends on the steps)
+    if (m <= SHORT) return std::max(size, short_workspace(batch, m, n));  // (which of the two it is depends on the steps)
+    return panel_fits(dtype, batch, m, n) ? panel_workspace(batch, m, n) : size;
 }
 
 extern "C" int lbfgs_train_orthogonalize(int32_t dtype, int64_t batch, int64_t rows, int64_t cols, const void* update, void* out, int32_t steps, double a, double b,
@@ -659,6 +652,15 @@ extern "C" int lbfgs_train_orthogonalize(int32_t dtype, int64_t batch, int64_t r
             case LBFGS_TRAIN_F32: short_orthogonalize<float>(p, s); break;
             case LBFGS_TRAIN_BF16: short_orthogonalize<bf16>(p, s); break;
             default: short_orthogonalize<f16>(p, s);
+        }
+        return lt_launched(who);
+    }
+    if (panel_fits(dtype, batch, q.m, q.n)) {
+        const Panel p = {update, out, workspace, q.m, q.n, q.tall, q.batch, q.steps, a, b, c, q.sx, q.ss, q.sp, norm_blocks(q)};
+        switch (dtype) {
+            case LBFGS_TRAIN_F32: launch_panels<float>(q, p, s); break;
+            case LBFGS_TRAIN_BF16: launch_panels<bf16>(q, p, s); break;
+            default: launch_panels<f16>(q, p, s);
         }
         return lt_launched(who);
     }

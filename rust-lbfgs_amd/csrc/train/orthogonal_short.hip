@@ -20,7 +20,6 @@
 
 namespace lt {
 
-typedef float float4_ __attribute__((ext_vector_type(4)));
 typedef double double4_ __attribute__((ext_vector_type(4)));
 
 // v_mfma_f64_16x16x4: lane l has row (column) l % 16 of L (of R), K = l / 16; of the result column l % 16, rows l / 16 + 4 r

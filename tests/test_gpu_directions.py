@@ -163,6 +163,29 @@ def test_more_steps_of_a_short_side_than_64_bits_have_room_for(steps, abc, dtype
     check(gradient(40, 300, dtype=DT[dtype], rank=40), steps, abc)
 
 
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("shape", [(65, 65), (65, 1000), (96, 97), (96, 1536), (96, 1537), (97, 512), (128, 129), (128, 513), (128, 768), (128, 769), (4096, 128), (4097, 100), (700, 66),
+                                   (30, 100, 500), (20, 70, 260), (2, 128, 130, 90), (300, 80, 90)])
+def test_a_side_of_up_to_128(shape, dtype):
+    """One launch a step, panels of 64 and 128 columns, and where that ends."""
+    g = gradient(*shape, dtype=DT[dtype])
+    got, _ = check(g) if g.numel() < 400000 else (directions.orthogonalize(g), check_large(g))
+    assert torch.equal(got, directions.orthogonalize(g))
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_bad_values_of_a_side_of_up_to_128_stay_with_their_matrix(dtype):
+    g = gradient(5, 130, 75, dtype=DT[dtype])
+    g[1] = 0
+    g[2, 129, 74] = math.nan
+    g[3, 0, 0] = -math.inf
+    got = directions.orthogonalize(g)
+    assert (got[1] == 0).all() and got[2].isnan().all() and got[3].isnan().all()
+    for k in (0, 4):
+        assert torch.equal(got[k], directions.orthogonalize(g[k]))
+        assert torch.equal(got[k].t(), directions.orthogonalize(g[k].t().contiguous()))
+
+
 def test_many_steps_of_a_short_side_and_no_full_rank():
     for shape in ((40, 300), (64, 64), (300, 20)):
         for dtype in DT.values():
