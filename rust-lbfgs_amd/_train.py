@@ -120,7 +120,7 @@ def ptr(t):
 
 def enqueue(function, device, *arguments):
     """`function(*arguments, stream)` with the tensors' device as the current one, on its current stream."""
-    if torch.cuda.current_device() == device.index:
+    if torch._C._cuda_getDevice() == device.index:  # (what torch.cuda.current_device() asks, once torch has started)
         rc = function(*arguments, torch._C._cuda_getCurrentRawStream(device.index))
     else:
         with torch.cuda.device(device):

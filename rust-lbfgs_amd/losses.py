@@ -41,12 +41,15 @@ def _rows(logits, targets, ignore_index):
     if not targets.is_contiguous():
         targets = targets.contiguous()
     x = logits
+    if x.is_contiguous():
+        v = x.shape[-1]
+        return _train.Rows(x.data_ptr(), targets.data_ptr(), _train.DTYPES[x.dtype], 0, 1, targets.numel(), v, 0, v, ignore_index), dev, (x, targets)
     n = x.dim()
     if n > 3:
         x = x.detach().flatten(0, -3)  # (a copy only if the leading dimensions have no common stride)
         n = 3
     shape, strides = x.shape, x.stride()
-    if (shape[-1] > 1 and strides[-1] != 1) or min(strides) < 0:
+    if shape[-1] > 1 and strides[-1] != 1:
         x = x.detach().contiguous()
         strides = x.stride()
     outer, outer_stride = (shape[0], strides[0]) if n == 3 else (1, 0)
@@ -64,7 +67,7 @@ def token_logprobs_with_lse(logits, targets, temperature=1.0, ignore_index=-100)
     row is not read; any other target outside [0, V) gives NaN.  Masked logits may be -inf or the type's lowest value."""
     rows, dev, keep = _rows(logits, targets, ignore_index)
     L = _train.load()
-    logps = logits.new_empty(targets.shape, dtype=_train.wide(logits.dtype))
+    logps = torch.empty_like(keep[1], dtype=_train.wide(logits.dtype))  # (the targets, dense)
     lse = logits.new_empty((*targets.shape, 2), dtype=torch.float64)
     size = L.lbfgs_train_token_logprobs_workspace(rows.dtype, rows.outer * rows.inner, rows.vocab)
     ws = logits.new_empty(size, dtype=torch.uint8) if size else None
