@@ -9,6 +9,7 @@
  *    calling thread's message.  Arguments are checked before anything is enqueued;
  *  - all pointers are device memory of ONE device, which is the calling thread's current one; nothing is allocated,
  *    copied to the host or waited for: a call only enqueues kernels, also into a stream that is being captured;
+ *  - outputs overlap neither inputs nor each other;
  *  - workspaces are the caller's, aligned to 256 bytes and at least as large as the matching *_workspace() says, one for each
  *    call in flight (calls on one stream may share one); their contents need no preparation and mean nothing afterwards;
  *  - element types: F64, F32, BF16, F16.  The wide type of a call is F64 for F64 data and F32 for the others: sums and

@@ -335,6 +335,7 @@ extern "C" int lbfgs_train_token_logprobs(const lbfgs_train_rows* rows, double t
     const uint64_t need = lbfgs_train_token_logprobs_workspace(rows->dtype, r.rows, r.vocab);
     if (need && (!workspace || workspace_bytes < need))
         return lt_fail(LBFGS_HIP_ERR_ARG, "%s: %llu bytes of workspace, %llu are needed", who, (unsigned long long)(workspace ? workspace_bytes : 0), (unsigned long long)need);
+    if (need && (uintptr_t)workspace % 256) return lt_fail(LBFGS_HIP_ERR_ARG, "%s: the workspace is not aligned to 256 bytes", who);
     hipStream_t s = (hipStream_t)stream;
     switch (rows->dtype) {
         case LBFGS_TRAIN_F64: launch_forward<double>(rows->logits, r, temperature, logps, lse, workspace, s); break;

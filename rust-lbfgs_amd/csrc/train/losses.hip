@@ -911,6 +911,7 @@ static int check_workspace(const void* workspace, uint64_t bytes, const Seqs& q,
     if (!need) return LBFGS_HIP_OK;
     if (!workspace || bytes < need)
         return lt_fail(LBFGS_HIP_ERR_ARG, "%s: %llu bytes of workspace, %llu are needed", who, (unsigned long long)(workspace ? bytes : 0), (unsigned long long)need);
+    if ((uintptr_t)workspace % 256) return lt_fail(LBFGS_HIP_ERR_ARG, "%s: the workspace is not aligned to 256 bytes", who);
     lay_out(sp, (void*)workspace, q.tokens, q.count);
     return LBFGS_HIP_OK;
 }

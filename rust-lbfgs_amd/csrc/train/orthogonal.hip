@@ -645,6 +645,7 @@ extern "C" int lbfgs_train_orthogonalize(int32_t dtype, int64_t batch, int64_t r
     const uint64_t need = lbfgs_train_orthogonalize_workspace(dtype, batch, rows, cols);
     if (!workspace || workspace_bytes < need)
         return lt_fail(LBFGS_HIP_ERR_ARG, "%s: %llu bytes of workspace, %llu are needed", who, (unsigned long long)(workspace ? workspace_bytes : 0), (unsigned long long)need);
+    if ((uintptr_t)workspace % 256) return lt_fail(LBFGS_HIP_ERR_ARG, "%s: the workspace is not aligned to 256 bytes", who);
     hipStream_t s = (hipStream_t)stream;
     if (q.brief) {
         const Short p = {update, out, workspace, q.m, q.n, q.tall, q.batch, q.steps, a, b, c};

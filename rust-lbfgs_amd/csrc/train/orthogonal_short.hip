@@ -10,8 +10,8 @@
 // Such updates are bound by latency: products of whole matrices, one launch each, take 4 to 5 us apiece, three a step.  Here there
 // are three launches in all: sums over slices of the long side, the steps, the result.  Measured, five steps, in us, with the
 // launches' own time, against products of the whole matrix: 32 x 64 27 (70), 64 x 128 48 (77), 64 x 1000 53 (100; bf16 83),
-// 64 x 4000 59 (179; bf16 107), 16 of 64 x 64 47 (75).  At 64 the steps alone take 30 us, 17 products of 64^3 at 2560 to 3072
-// cycles of the matrix units and as much for reads of LDS, sums and barriers; at 32 10, at 16 5.  Sides beyond 64 would not fit the
+// 64 x 4000 59 (179; bf16 107), 16 of 64 x 64 47 (75).  At 64 the steps alone take 30 us, 17 products of 64^3 at 1.1 to 1.3 us
+// of the matrix units and half as much for reads of LDS, sums and barriers; at 32 10, at 16 5.  Sides beyond 64 would not fit the
 // LDS, and 128 x 128 in one compute unit would take 8 times as long.  The slices take 3 us at 16 x 64, 6 at 64 x 64, 15 at 64 x 5000, the
 // result 3, 9 and 10: both wait for memory and for each other's launches.
 #include "orthogonal.h"

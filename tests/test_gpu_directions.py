@@ -315,6 +315,29 @@ def test_captured_and_replayed():
         torch.ones(1000, device="cuda").sum()
 
 
+def test_captured_and_replayed_with_short_sides():
+    shapes = [(40, 700), (3, 64, 50), (100, 300), (2, 700, 90), (20, 9000)]
+    g = [gradient(*shape, seed=k) for k, shape in enumerate(shapes)]
+    for x in g:
+        directions.orthogonalize(x)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = [directions.orthogonalize(x) for x in g]
+        graphs.append((graph, out))
+    for k in range(4):
+        for n, x in enumerate(g):
+            x.copy_(gradient(*shapes[n], seed=10 * k + n + 3))
+        want = [directions.orthogonalize(x) for x in g]
+        for graph, out in graphs:
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+        torch.ones(1000, device="cuda").sum()
+
+
 def test_refusals_raise():
     g = gradient(10, 10)
     with pytest.raises(LbfgsError, match="steps"):

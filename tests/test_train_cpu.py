@@ -105,6 +105,7 @@ def test_c_logprobs_refusals(lib):
     assert need > 0 and lib.lbfgs_train_token_logprobs_workspace(2, 100000, 400000) == 0
     refused(lib.lbfgs_train_token_logprobs(rows(dtype=2, vocab=400000), 1.0, P, P, P, need - 1, None), "workspace")
     refused(lib.lbfgs_train_token_logprobs(rows(dtype=2, vocab=400000), 1.0, P, P, None, need, None), "workspace")
+    refused(lib.lbfgs_train_token_logprobs(rows(dtype=2, vocab=400000), 1.0, P, P, P + 128, 1 << 30, None), "aligned")
     assert lib.lbfgs_train_token_logprobs(rows(outer=0), 1.0, None, None, None, 0, None) == 0  # no rows: nothing to do
 
 
@@ -133,6 +134,7 @@ def test_c_preference_refusals(lib):
     need = lib.lbfgs_train_sequences_workspace(100000, 4)
     refused(call(seqs(tokens=100000), size=need - 1), "workspace")
     refused(call(seqs(tokens=100000), ws=None), "workspace")
+    refused(call(seqs(tokens=100000), ws=P + 8), "aligned")
 
 
 def test_c_policy_refusals(lib):
@@ -166,6 +168,7 @@ def test_c_orthogonalize_refusals(lib):
     refused(call(abc=(-8.0, 0.0, 4000.0)), "out of range")
     refused(call(g=None), "are needed")
     refused(call(ws=None), "workspace")
+    refused(call(ws=P + 64), "aligned")
     refused(call(size=lib.lbfgs_train_orthogonalize_workspace(1, 1, 4, 4) - 1), "workspace")
     assert lib.lbfgs_train_orthogonalize_workspace(1, 0, 4, 4) == lib.lbfgs_train_orthogonalize_workspace(0, 1, 4, 4) == 0
     assert call(batch=0, g=None, out=None, ws=None) == 0 and call(m=0, g=None, out=None, ws=None) == 0
