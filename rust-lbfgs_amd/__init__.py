@@ -14,7 +14,7 @@ from .api import (BuiltinObjective, Context, DeviceEvaluate, TorchEvaluate, Lbfg
 
 
 def build(force=False):
-    """Compile liblbfgs_hip.so and liblbfgs_train.so (hipcc, gfx950) and liblbfgs_solver.so (g++) in-tree."""
+    """Compile liblbfgs_hip.so and liblbfgs_train.so (hipcc, gfx950), liblbfgs_solver.so and liblbfgs_train_calls.so (g++) in-tree."""
     return _build.build_all(force)
 
 

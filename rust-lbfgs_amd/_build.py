@@ -4,6 +4,7 @@
                       csrc/context.hip, csrc/lbfgs_hip.hip, csrc/lj.hip, sharing csrc/ctx.h)
   liblbfgs_solver.so  host orchestration of include/lbfgs_solver.h    (g++, links the former)
   liblbfgs_train.so   loss and update operators of include/lbfgs_train.h   (hipcc, gfx950; the units of csrc/train)
+  liblbfgs_train_calls.so   their ordinary calls from Python                (g++ against torch's headers; csrc/train/calls.cpp)
 
 hipcc cross-compiles for gfx950 without a GPU.  -ffp-contract=off on both sides: the
 reference's arithmetic is mul-then-add with separate roundings (src/math.rs:35,41).
@@ -14,9 +15,11 @@ whenever that differs from the hash of the checked-out sources.  Modification ti
 """
 import glob
 import hashlib
+import importlib.util
 import os
 import re
 import subprocess
+import sysconfig
 import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -25,6 +28,7 @@ CSRC = os.path.join(HERE, "csrc")
 HIP_LIB = os.path.join(HERE, "liblbfgs_hip.so")
 SOLVER_LIB = os.path.join(HERE, "liblbfgs_solver.so")
 TRAIN_LIB = os.path.join(HERE, "liblbfgs_train.so")
+CALLS_LIB = os.path.join(HERE, "liblbfgs_train_calls.so")  # a Python extension: losses.py's and directions.py's ordinary calls
 TRAIN_RESOURCES = os.path.join(HERE, "liblbfgs_train.resources.txt")
 RESOURCES = os.path.join(HERE, "liblbfgs_hip.resources.txt")  # per-kernel register / scratch usage of the last build
 
@@ -40,6 +44,7 @@ SOLVER_SRCS = [os.path.join(CSRC, "host", "solver.cpp"), os.path.join(ROOT, "inc
 TRAIN_UNITS = [os.path.join(CSRC, "train", f) for f in ("losses.hip", "logprobs.hip", "orthogonal.hip", "orthogonal_short.hip", "orthogonal_panel.hip")]
 TRAIN_SRCS = TRAIN_UNITS + [os.path.join(CSRC, "train", "common.h"), os.path.join(CSRC, "train", "orthogonal.h"), os.path.join(ROOT, "include", "lbfgs_train.h"),
                             os.path.join(ROOT, "include", "lbfgs_hip.h")]
+CALLS_SRCS = [os.path.join(CSRC, "train", "calls.cpp"), os.path.join(ROOT, "include", "lbfgs_train.h"), os.path.join(ROOT, "include", "lbfgs_hip.h")]
 
 
 def source_hash(paths, flags=()):
@@ -71,6 +76,7 @@ HIP_FLAGS = ["-O3", "--offload-arch=gfx950", "-ffp-contract=off", "-fPIC", "-std
              "-mllvm", "-amdgpu-spill-vgpr-to-agpr=0", "-Wall"]
 # (32-bit arithmetic one value at a time: the packed forms the compiler makes by itself have given wrong results now and then)
 TRAIN_FLAGS = ["-O3", "--offload-arch=gfx950", "-fPIC", "-std=c++17", "-Wall", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+CALLS_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall"]
 SOLVER_FLAGS = ["-O2", "-ffp-contract=off", "-fPIC", "-shared", "-std=c++17", "-Wall"]
 
 
@@ -81,6 +87,18 @@ def hip_build_id():
 
 def train_build_id():
     return source_hash(TRAIN_SRCS, TRAIN_FLAGS)
+
+
+def _torch():
+    """-> (torch's folder, its version), without importing it."""
+    where = importlib.util.find_spec("torch").submodule_search_locations[0]
+    with open(os.path.join(where, "version.py")) as f:
+        return where, re.search(r"__version__ = '([^']+)'", f.read()).group(1)
+
+
+def calls_build_id():
+    """Of the Python extension: its sources, and the torch and the Python that it is compiled for."""
+    return source_hash(CALLS_SRCS, CALLS_FLAGS + [_torch()[1], sysconfig.get_python_version()])
 
 
 def solver_build_id():
@@ -204,8 +222,24 @@ def build_train(force=False):
     return TRAIN_LIB
 
 
+def build_calls(force=False):
+    want = calls_build_id()
+    if force or _stale(CALLS_LIB, "LBFGS_TRAIN_CALLS_BUILD_ID", want):
+        torch = _torch()[0]
+        include = [os.path.join(torch, "include"), os.path.join(torch, "include", "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"]]
+        _run(["g++", *CALLS_FLAGS, '-DLBFGS_TRAIN_CALLS_BUILD_ID="%s"' % want, *[f for i in include for f in ("-isystem", i)], CALLS_SRCS[0], "-o", CALLS_LIB,
+              "-L" + os.path.join(torch, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"])
+        if embedded_id(CALLS_LIB, "LBFGS_TRAIN_CALLS_BUILD_ID") != want:
+            raise RuntimeError("build: %s does not carry the id it was built with" % CALLS_LIB)
+        LAST_BUILD["liblbfgs_train_calls.so"] = "compiled"
+    else:
+        LAST_BUILD.setdefault("liblbfgs_train_calls.so", "reused")
+    return CALLS_LIB
+
+
 def build_all(force=False):
     build_train(force)
+    build_calls(force)
     return build_hip(force), build_solver(force)
 
 

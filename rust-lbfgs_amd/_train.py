@@ -1,5 +1,5 @@
-"""ctypes declarations of include/lbfgs_train.h, and what losses.py and directions.py share: the loader of
-liblbfgs_train.so and the checks of torch tensors.
+"""ctypes declarations of include/lbfgs_train.h, and what losses.py and directions.py share: the loaders of
+liblbfgs_train.so and of the extension that makes their ordinary calls, and the checks of torch tensors.
 
 The operators take tensors of the GPU and enqueue HIP kernels on the tensors' device and its current stream, as torch's own
 operators do.  There is no CPU fallback: without the built library, or with tensors elsewhere, they raise.
@@ -7,6 +7,8 @@ operators do.  There is no CPU fallback: without the built library, or with tens
 from __future__ import annotations
 
 import ctypes as C
+import importlib.machinery
+import importlib.util
 import os
 
 import torch  # before the library: it has to bind to torch's HIP runtime
@@ -72,9 +74,44 @@ def load():
     return lib
 
 
+_CALLS = None
+
+
+def calls():
+    """The extension liblbfgs_train_calls.so: a function for each operator that does the whole of an ordinary call -- tensors that are dense,
+    of the right types and shapes and on the current device -- and returns its results, or the status of a refused one, or None: it has done
+    nothing, and the operator's own checks follow.  Raises if it is not built, or built from other sources or for another torch."""
+    global _CALLS
+    if _CALLS is not None:
+        return _CALLS
+    lib, path = load(), _build.CALLS_LIB
+    if not os.path.exists(path):
+        raise ImportError(f"{path} is missing: the extension is not built (python -c 'import rust_lbfgs_amd as r; r.build()')")
+    have, want = _build.embedded_id(path, "LBFGS_TRAIN_CALLS_BUILD_ID"), _build.calls_build_id()
+    if have != want and os.environ.get("LBFGS_HIP_ALLOW_STALE") != "1":
+        raise ImportError(f"{path} carries build id {have}, the checked-out sources and this torch hash to {want}: rebuild "
+                          "(python -c 'import rust_lbfgs_amd as r; r.build()'), or set LBFGS_HIP_ALLOW_STALE=1 to load it anyway")
+    loader = importlib.machinery.ExtensionFileLoader("liblbfgs_train_calls", path)
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader(loader.name, loader))
+    loader.exec_module(module)
+    functions = [C.cast(getattr(lib, "lbfgs_train_" + name), C.c_void_p).value for name in (
+        "token_logprobs_workspace", "token_logprobs", "token_logprobs_grad", "sequences_workspace", "preference", "policy", "orthogonalize_workspace", "orthogonalize")]
+    # (the current stream of a device, as a number; on a build of torch without a GPU there is none to ask for, nor a tensor that would need it)
+    module.bind(*functions, getattr(torch._C, "_cuda_getCurrentRawStream", None))
+    _CALLS = module
+    return module
+
+
 def check(rc):
     if rc != 0:
         _raise(rc, load().lbfgs_train_last_error().decode())
+
+
+def results(done):
+    """What a native call left: its results, or the status of a refused one."""
+    if type(done) is not tuple:
+        check(done)
+    return done
 
 
 def wide(dtype):

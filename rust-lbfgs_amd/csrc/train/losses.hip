@@ -782,20 +782,35 @@ __global__ __launch_bounds__(BLOCK) void policy_small_kernel(Seqs whole, Policy 
         if (w < chunks) t[w].get(x, whole.mask, o.per_token, w * CHUNK + threadIdx.x * E, whole.tokens);
     const SmallSeqs q = small_seqs(whole, m, sp);
     __syncthreads();
-    if (q.mask) {
+    double kept, some = 1, f = 0, kl = 0, clipped = 0;
+    if (!o.by_sequence) {  // the number of all tokens is wanted, not each sequence's
+        int n = 0;
+        bool bad = false;
 #pragma unroll
         for (int w = 0; w < SMALL_CHUNKS; w++)
-            if (w < chunks) {
-                Tokens<T> k;
-                k.keep = t[w].keep;
-                chunk_sums(q, k, false, false, w, sp);
+#pragma unroll
+            for (int k = 0; k < E; k++) {
+                const int at = w * CHUNK + (int)threadIdx.x * E + k;
+                if (w < chunks && at >= q.at(0) && at < q.at(q.count)) n += t[w].keep.v[k] != 0;
             }
+        for (int64_t s = threadIdx.x; s < q.count; s += BLOCK) bad |= !q.good(s);
+        kept = block_sum(bad ? NAN : (double)n);
+        if (kept < 1) kept = 1;
+    } else {
+        if (q.mask) {
+#pragma unroll
+            for (int w = 0; w < SMALL_CHUNKS; w++)
+                if (w < chunks) {
+                    Tokens<T> k;
+                    k.keep = t[w].keep;
+                    chunk_sums(q, k, false, false, w, sp);
+                }
+            __syncthreads();
+        }
+        sequence_weights(q, sp, 0, 1);
         __syncthreads();
+        all_counts(sp, 1, kept, some);
     }
-    sequence_weights(q, sp, 0, 1);
-    __syncthreads();
-    double kept, some, f = 0, kl = 0, clipped = 0;
-    all_counts(sp, 1, kept, some);
     const double inv = 1.0 / (o.by_sequence ? some : kept);
 #pragma unroll
     for (int w = 0; w < SMALL_CHUNKS; w++)
@@ -804,9 +819,9 @@ __global__ __launch_bounds__(BLOCK) void policy_small_kernel(Seqs whole, Policy 
 }
 
 // ------------------------------------------------------------------------------------ launches
-// Up to so many tokens and sequences one workgroup does the whole of a loss, without a workspace.  Measured, kernels alone, in us:
-// 8 sequences of 60 tokens, preference 7.0 (8.2 as several launches), policy 7.2 (10.9); 64 of 64, preference 11.0 (8.2), policy 11.3
-// (11.7); the launches saved, one and two, and the workspace take 4 to 8 us of the host, which is what such a call takes.
+// Up to so many tokens and sequences one workgroup does the whole of a loss, without a workspace.  Measured, whole calls one after the
+// other, in us (as several launches in brackets): 8 sequences of 60 tokens, preference 7.4 (10.3), policy 7.5 (13.7); 2 of 2048, 9.2 (10.3)
+// and 9.7 (13.8), with a mask and a mean of means 13.0 (16.5); 256 of 16, 11.0 (10.3), 12.2 (13.8) and 17.9 (16.8).
 static bool small(int64_t tokens, int64_t seqs) { return tokens <= SMALL_TOKENS && seqs <= SMALL_SEQS; }
 
 static int64_t chunks_of(int64_t tokens) { return (tokens + CHUNK - 1) / CHUNK; }

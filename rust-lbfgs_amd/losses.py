@@ -65,6 +65,9 @@ def token_logprobs_with_lse(logits, targets, temperature=1.0, ignore_index=-100)
     -> (logps [...] in float64 for float64 logits, else float32; lse [..., 2] float64: each row's largest logit m and
     log sum exp((logits - m) / temperature), the two parts of its log-sum-exp m / temperature + that).  A target `ignore_index` gives 0 and its
     row is not read; any other target outside [0, V) gives NaN.  Masked logits may be -inf or the type's lowest value."""
+    done = _train.calls().logprobs(logits, targets, temperature, ignore_index)
+    if done is not None:
+        return _train.results(done)
     rows, dev, keep = _rows(logits, targets, ignore_index)
     L = _train.load()
     logps = torch.empty_like(keep[1], dtype=_train.wide(logits.dtype))  # (the targets, dense)
@@ -81,6 +84,9 @@ def token_logprobs_grad(logits, targets, lse, grad, temperature=1.0, ignore_inde
 
     `lse` and the other arguments are those of token_logprobs_with_lse; `grad` [...] is df/dlogps in its type.  Rows whose
     grad is 0 are not read."""
+    done = _train.calls().logprobs_grad(logits, targets, lse, grad, temperature, ignore_index)
+    if done is not None:
+        return _train.results(done)[0]
     rows, dev, keep = _rows(logits, targets, ignore_index)
     _train.like("lse", lse, "logits", torch.float64, (*targets.shape, 2))
     _train.like("grad", grad, "logits", _train.wide(logits.dtype), targets.shape)
@@ -165,6 +171,9 @@ def preference(logps, ref_logps=None, *, offsets=None, mask=None, beta=0.1, kind
     All sums are taken in 64 bits.  -> Preference(f, rewards, grad); f and rewards in float64 for float64 data, else float32."""
     if kind not in KINDS:
         raise ValueError(f"kind must be one of {', '.join(KINDS)}, not {kind!r}")
+    done = _train.calls().preference(logps, ref_logps, offsets, mask, beta, label_smoothing, KINDS[kind], normalize_lengths)
+    if done is not None:
+        return Preference._make(_train.results(done))
     others = (("ref_logps", ref_logps),)
     q, count, (x, m, o, ref) = _sequences(logps, offsets, mask, others)
     dev = _train.on_gpu("logps", logps, (("offsets", offsets), ("mask", mask), *others))
@@ -196,6 +205,9 @@ def policy(logps, old_logps, advantages, *, ref_logps=None, offsets=None, mask=N
         raise ValueError(f"reduction must be one of {', '.join(REDUCTIONS)}, not {reduction!r}")
     if kl_coef != 0 and ref_logps is None:
         raise ValueError("a KL term needs ref_logps")
+    done = _train.calls().policy(logps, old_logps, advantages, ref_logps, offsets, mask, clip_low, clip_high, kl_coef, REDUCTIONS[reduction])
+    if done is not None:
+        return Policy._make(_train.results(done))
     others = (("old_logps", old_logps), ("ref_logps", ref_logps))
     q, count, (x, m, o, old, ref) = _sequences(logps, offsets, mask, others)
     per_token = not (isinstance(advantages, torch.Tensor) and advantages.shape == (count, 1))

@@ -565,6 +565,51 @@ def test_captured_and_replayed():
         torch.ones(1000, device="cuda").sum()
 
 
+def test_native_calls_and_the_way_through_python_agree(monkeypatch):
+    """What the native calls decline goes through Python's checks and copies to the same kernels."""
+    from rust_lbfgs_amd import _train, directions
+
+    lp, other, off, mask, _, _ = ragged([5, 0, 1, 17, 3, 2], torch.float32, 3, "packed", 0.3)
+    x, y, g = make((3, 4), 1000, torch.bfloat16)
+    w = torch.randn(3, 30, 50, generator=torch.Generator().manual_seed(1)).cuda()
+    A = torch.randn(6, 1, generator=torch.Generator().manual_seed(2)).cuda()
+
+    def everything():
+        out = list(losses.token_logprobs_with_lse(x, y, 0.7, -1))
+        out.append(losses.token_logprobs_grad(x, y, out[1], g, 0.7, -1))
+        out += losses.preference(lp, other, offsets=off, mask=mask, beta=0.2, kind="squared", normalize_lengths=True)
+        out += losses.policy(lp, other, A, ref_logps=other, offsets=off.int(), mask=mask, clip_low=0.1, clip_high=math.inf, kl_coef=0.1, reduction="sequences")
+        out += losses.policy(lp.half().view(1, -1), other.half().view(1, -1), lp.half().view(1, -1), mask=mask.view(1, -1))
+        return out + [directions.orthogonalize(w, steps=4, coefficients=(2, -1.5, 0.5))]
+
+    native = everything()
+    real = _train.calls()
+    names = [n for n in dir(real) if not n.startswith("_")]
+    declined = type("Declined", (), {n: staticmethod(lambda *a: None) for n in names})
+    asked = []
+    counting = type("Counting", (), {n: staticmethod(lambda *a, n=n: (asked.append(n), getattr(real, n)(*a))[1]) for n in names})
+    monkeypatch.setattr(_train, "_CALLS", counting)
+    done = everything()
+    assert asked == ["logprobs", "logprobs_grad", "preference", "policy", "policy", "orthogonalize"]
+    monkeypatch.setattr(_train, "_CALLS", declined)
+    for a, b, c in zip(native, done, everything()):
+        assert a.dtype == c.dtype and a.shape == c.shape and torch.equal(a.nan_to_num(7.0), c.nan_to_num(7.0)) and torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0))
+
+
+def test_no_memory_is_torchs_own_error():
+    x = torch.zeros(1 << 20, 65, dtype=torch.bfloat16, device="cuda")
+    before = torch.cuda.memory_allocated()
+    torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (64 << 20)) / torch.cuda.get_device_properties(0).total_memory)
+    try:
+        from rust_lbfgs_amd import directions
+
+        with pytest.raises(torch.OutOfMemoryError):
+            directions.orthogonalize(x)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert torch.cuda.memory_allocated() == before and losses.preference(torch.zeros(2, 3, device="cuda")).f.isfinite()
+
+
 def test_autograd_forms_refuse_a_capture():
     x, y, ref, mask = three(0)
     x.requires_grad_()

@@ -20,6 +20,8 @@ P = 4096  # a pointer that is not null; no refused call looks at it
 def lib():
     if not os.path.exists(_build.TRAIN_LIB):
         _build.build_train()
+    if not os.path.exists(_build.CALLS_LIB):
+        _build.build_calls()
     return _train.load()
 
 
@@ -255,6 +257,38 @@ def test_views_with_a_sign_to_come_are_refused(lib):
                  lambda: losses.policy(torch.ones(6), torch.ones(6), lazy, offsets=off), lambda: directions.orthogonalize(lazy.view(2, 3))):
         with pytest.raises(TypeError, match="resolve_neg"):
             call()
+
+
+def test_native_calls_decline_what_is_not_ordinary(lib):
+    """Tensors that are elsewhere, of other types or shapes, or no tensors at all: None, and nothing done."""
+    c = _train.calls()
+    x, y, g = torch.zeros(2, 8), torch.zeros(2, dtype=torch.int64), torch.zeros(2)
+    for a in ((x, y, 1.0, -100), (None, y, 1.0, -100), (x, 3, 1.0, -100), (x, y, "1", -100), (x, y, 1.0, 1 << 70), ("x", y, 1, -100)):
+        assert c.logprobs(*a) is None
+    assert c.logprobs_grad(x, y, torch.zeros(2, 2, dtype=torch.float64), g, 1.0, -100) is None
+    for off, mask in ((None, None), (torch.tensor([0, 1]), None), (7, x), ("a", 1)):
+        assert c.preference(x, x, off, mask, 0.1, 0.0, 0, False) is None
+        assert c.policy(x, x, x, None, off, mask, 0.2, 0.2, 0.0, 0) is None
+    assert c.orthogonalize(x, 5, 1.0, 2.0, 3.0) is None and c.orthogonalize(None, 5, 1.0, 2.0, 3.0) is None
+    assert c.orthogonalize(x.to_sparse(), 5, 1.0, 2.0, 3.0) is None and c.orthogonalize(torch.zeros(2, 3, device="meta"), 5, 1.0, 2.0, 3.0) is None
+    for f, n in ((c.logprobs, 4), (c.logprobs_grad, 6), (c.preference, 8), (c.policy, 10), (c.orthogonalize, 5), (c.bind, 9)):
+        for k in (0, n - 1, n + 1):
+            with pytest.raises(TypeError, match=f"{n} are taken"):
+                f(*[x] * k)
+
+
+def test_the_native_calls_are_rebuilt_when_sources_or_torch_differ(lib, monkeypatch):
+    assert _build.embedded_id(_build.CALLS_LIB, "LBFGS_TRAIN_CALLS_BUILD_ID") == _build.calls_build_id()
+    assert _build._torch()[1] == torch.__version__
+    before = _build.calls_build_id()
+    monkeypatch.setattr(_build, "_torch", lambda: (os.path.dirname(torch.__file__), "0.0"))
+    assert _build.calls_build_id() != before
+    monkeypatch.setattr(_train, "_CALLS", None)
+    with pytest.raises(ImportError, match="build id"):
+        _train.calls()
+    monkeypatch.setattr(_build, "CALLS_LIB", "/nowhere.so")
+    with pytest.raises(ImportError, match="missing"):
+        _train.calls()
 
 
 def test_modules_are_reached_from_the_package():
