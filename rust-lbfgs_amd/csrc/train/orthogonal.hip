@@ -353,12 +353,16 @@ __global__ __launch_bounds__(WAVES * WAVE, TILE <= 128 && STAGES * TILE <= 256 ?
         for (int y = 0; y < NJ; y++) {
             const float4_ v = PARTS == 3 ? acc[x][y] + low[x][y] : acc[x][y];
             const int i = wi + x * 16 + (lane / 16) * 4, j = wj + y * 16 + lane % 16;
-            if (!diagonal)
-                *(float4_*)&res[spot(i, j)] = v;
-            else if (wi + x * 16 >= wj + y * 16)
+            const int below = wi + x * 16 - (wj + y * 16);
+            if (!diagonal || below > 0) *(float4_*)&res[spot(i, j)] = v;
+            if (diagonal && below > 0) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) res[spot(j, i + e)] = v[e];
+            } else if (diagonal && below == 0) {
 #pragma unroll
                 for (int e = 0; e < 4; e++)
                     if (i + e >= j) res[spot(i + e, j)] = res[spot(j, i + e)] = v[e];
+            }
         }
     __syncthreads();
     float scale = p.scale;
