@@ -648,32 +648,32 @@ struct PolicyTokens {
     }
 };
 
-// L = -min(r A, clip(r) A) + kl (e^q - 1 - q) with r = e^d, d = logp - old, q = ref - logp.  Products with A and sums are taken in 64
-// bits: advantages have mean 0, and the mean of r A is what is left of terms a thousand times larger.
+// L = -min(r A, clip(r) A) + kl (e^q - 1 - q) with r = e^d, d = logp - old, q = ref - logp.  Products with A, sums and the slope are taken in 64
+// bits (the slope is rounded once, to the gradient's type): advantages have mean 0, and the mean of r A is what is left of terms a thousand
+// times larger.
 template <class T>
-__device__ __forceinline__ void token(const Policy& o, T lp, T old, T ref, double a, double weight, typename Num<T>::acc& slope, double& f, double& kl, double& clipped) {
+__device__ __forceinline__ void token(const Policy& o, T lp, T old, T ref, double a, double weight, double& slope, double& f, double& kl, double& clipped) {
     typedef typename Num<T>::acc A;
     bool over;
     double ra;
     ratio(o, (A)lp, (A)old, a, over, ra);
     double loss = over ? -(a > 0 ? o.high : o.low) * a : -ra;
-    slope = over ? (A)0 : (A)-ra;
+    slope = over ? 0 : -ra;
     if (o.kl != 0) {
         A em1, term;
         kl_terms((A)ref - (A)lp, em1, term);
         loss += o.kl * (double)term;
-        slope -= (A)o.kl * em1;
+        slope -= o.kl * (double)em1;
         kl += (double)term;
     }
     f += loss * weight;
     clipped += over;
-    slope *= (A)weight;
+    slope *= weight;
 }
 
 template <class T, class Q>
 __device__ __forceinline__ void chunk_policy(const Q& q, const Policy& o, const PolicyTokens<T>& x, const T* advantages, T* grad, const double* inverse, double inv,
                                              int64_t w, double& f, double& kl, double& clipped) {
-    typedef typename Num<T>::acc A;
     const int64_t t0 = w * CHUNK + threadIdx.x * E, n = q.tokens;
     Spot at = q.locate(t0);
     if (t0 >= n) return;
@@ -688,7 +688,7 @@ __device__ __forceinline__ void chunk_policy(const Q& q, const Policy& o, const 
     enter();
 #pragma unroll
     for (int k = 0; k < E; k++) {
-        A slope = 0;
+        double slope = 0;
         if (k >= at.begin && k < at.end && x.keep.v[k])
             token<T>(o, x.lp.v[k], x.old.v[k], x.ref.v[k], o.per_token ? (double)x.adv.v[k] : a_seq, weight, slope, f, kl, clipped);
         g.v[k] = (T)slope;
@@ -730,7 +730,6 @@ __global__ __launch_bounds__(BLOCK) void policy_kernel(Seqs q, Policy o, PolicyD
 constexpr int ALIKE_BLOCKS = 1280;  // five to a compute unit
 template <class T>
 __global__ __launch_bounds__(BLOCK) void policy_alike_kernel(Seqs q, Policy o, PolicyData<T> x, int count_blocks, Space sp) {
-    typedef typename Num<T>::acc A;
     constexpr int N = vec_len<T>();
     double kept, some, f = 0, kl = 0, clipped = 0;
     all_counts(sp, count_blocks, kept, some);
@@ -745,17 +744,17 @@ __global__ __launch_bounds__(BLOCK) void policy_alike_kernel(Seqs q, Policy o, P
             if (q.mask) keep = *(const Pack<uint8_t, N>*)(q.mask + t);
 #pragma unroll
             for (int k = 0; k < N; k++) {
-                A slope = 0;
+                double slope = 0;
                 if (t + k >= begin && t + k < end && (!q.mask || keep.v[k])) token<T>(o, lp.v[k], old.v[k], ref.v[k], (double)adv.v[k], 1.0, slope, f, kl, clipped);
-                g.v[k] = (T)(slope * (A)inv);
+                g.v[k] = (T)(slope * inv);
             }
             *(Pack<T, N>*)(x.grad + t) = g;
         } else {
             for (int64_t k = t; k < n; k++) {
-                A slope = 0;
+                double slope = 0;
                 if (k >= begin && k < end && (!q.mask || q.mask[k]))
                     token<T>(o, x.logps[k], x.old[k], x.ref ? x.ref[k] : (T)0, (double)x.adv[k], 1.0, slope, f, kl, clipped);
-                x.grad[k] = (T)(slope * (A)inv);
+                x.grad[k] = (T)(slope * inv);
             }
         }
     }
