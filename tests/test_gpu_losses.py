@@ -458,6 +458,25 @@ def test_bad_offsets_give_nan(bits):
     assert losses.preference(lp, offsets=o).f.isfinite()
 
 
+def test_losses_beyond_32_bits():
+    """More than 2^31 tokens; the second sequence reaches over all of them."""
+    n = 2 ** 31 + 4099
+    x = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    x[2], x[-1], x[n - 5000] = 1.0, -2.0, -4.0
+    off = torch.tensor([0, 5, n], device="cuda")
+    r = losses.preference(x, offsets=off, beta=0.5)
+    slope = -0.5 / (1 + math.exp(3.5))  # h = 0.5 (1 - (-6))
+    assert abs(float(r.f) - math.log1p(math.exp(-3.5))) < 1e-8 and r.rewards.tolist() == [0.5, -3.0]
+    want = torch.tensor([slope, -slope]).to(torch.bfloat16).cuda()
+    assert (r.grad[:5] == want[0]).all() and bool((r.grad[5:] == want[1]).all())
+    del r
+    p = losses.policy(x, x, x, offsets=off)  # every ratio is 1: f = -mean A, the gradient -A / N
+    assert abs(float(p.f) - 5.0 / n) < 1e-15 and float(p.clip_fraction) == 0
+    assert bool((p.grad.count_nonzero() == 3).all()) and abs(float(p.grad[-1]) * n - 2.0) < 2 * 2.0 ** -8
+    p = losses.policy(x, x, torch.tensor([[1.0], [2.0]], device="cuda").bfloat16(), offsets=off, reduction="sequences")
+    assert abs(float(p.f) + 1.5) < 1e-6 and abs(float(p.grad[-1]) * (n - 5) + 1.0) < 2.0 ** -7 and abs(float(p.grad[0]) * 5 + 0.5) < 2.0 ** -8
+
+
 def test_losses_take_strided_tensors():
     base = -torch.rand(6, 40, 2).cuda()
     lp, old = base[:, 1:, 0], base[:, :-1, 1]
