@@ -4,8 +4,8 @@
 //
 // Both are bound by HBM: the forward pass reads every logit once (running maximum and sum in registers), the gradient
 // reads it once more and writes as much.  Measured in bf16 (a copy of 2 GiB: 4.93 TB/s, read and written): 8192 x 131072 forward
-// 347 us, 6.2 TB/s; 8192 x 32768 forward 111 us, 4.8 TB/s, gradient 176 us, 6.1 TB/s, part of what it reads being in the caches yet;
-// rows of odd length in 32 bits, 16-byte loads at any alignment, 5.2 TB/s.  Few rows are bound by the launch: 8 rows of 32768 5 us.
+// 347 us, 6.2 TB/s; 8192 x 32768 forward 79 to 110 us, 4.8 TB/s and more, gradient 173 us, 6.2 TB/s, part of what both read being in the
+// caches yet; 1020 rows of 50001 in 32 bits, 16-byte loads at any alignment, 28 and 56 us.  Few rows are bound by the launch: 8 of 32768 5.
 #include "common.h"
 
 #include <algorithm>
@@ -168,7 +168,18 @@ __global__ __launch_bounds__(WAVE) void logprobs_join_kernel(const T* x, Rows r,
 }
 
 // The gradient: element-wise once the row's maximum and sum are known, so a row is cut into as many parts as fill the chip.
-template <class T, int N, class A>
+// 16 bytes of it; PAST: by the caches, which a gradient of this size would empty of the logits that are to be read yet
+typedef uint32_t uint4_ __attribute__((ext_vector_type(4)));
+// (compiled apart: two stores to one place on either side of a branch become one, of the ordinary kind)
+template <bool PAST, class T, int N>
+__device__ __forceinline__ void put(T* dx, const Pack<T, N>& d) {
+    uint4_* const to = (uint4_*)__builtin_assume_aligned(dx, 16);
+    if (PAST)
+        __builtin_nontemporal_store(*(const uint4_*)&d, to);
+    else
+        *to = *(const uint4_*)&d;
+}
+template <bool PAST, class T, int N, class A>
 __device__ __forceinline__ void grad_pack(const Pack<T, N>& p, T* dx, int64_t v, int64_t y, A hi, A c, A scale, A at_target) {
     Pack<T, N> d;
 #pragma unroll
@@ -182,10 +193,10 @@ __device__ __forceinline__ void grad_pack(const Pack<T, N>& p, T* dx, int64_t v,
     if (N == 1)
         dx[v] = d.v[0];
     else
-        *(Pack<T, N>*)__builtin_assume_aligned(dx + v, 16) = d;
+        put<PAST>(dx + v, d);
 }
 
-template <class T, int BLOCK>
+template <class T, int BLOCK, bool PAST>
 __global__ __launch_bounds__(BLOCK) void logprobs_grad_kernel(const T* x, Rows r, double tau, typename Num<T>::acc c, int splits, int64_t part,
                                                               const double* lse, const typename Num<T>::acc* grad, T* dx) {
     typedef typename Num<T>::acc A;
@@ -205,7 +216,7 @@ __global__ __launch_bounds__(BLOCK) void logprobs_grad_kernel(const T* x, Rows r
                 Pack<T, N> z;
 #pragma unroll
                 for (int k = 0; k < N; k++) z.v[k] = (T)0;
-                *(Pack<T, N>*)__builtin_assume_aligned(out + head + i * N, 16) = z;
+                put<PAST>(out + head + i * N, z);
             }
             for (int64_t k = lo + tid; k < head; k += BLOCK) out[k] = (T)0;
             for (int64_t k = done + tid; k < hi_v; k += BLOCK) out[k] = (T)0;
@@ -225,15 +236,18 @@ __global__ __launch_bounds__(BLOCK) void logprobs_grad_kernel(const T* x, Rows r
 #pragma unroll
             for (int u = 0; u < U; u++) p[u] = *(const Pack<T, N>*)(in + head + (i + u * BLOCK) * N);
 #pragma unroll
-            for (int u = 0; u < U; u++) grad_pack<T, N, A>(p[u], out, head + (i + u * BLOCK) * N, y, hi, c, scale, at_target);
+            for (int u = 0; u < U; u++) grad_pack<PAST, T, N, A>(p[u], out, head + (i + u * BLOCK) * N, y, hi, c, scale, at_target);
         }
-        for (; i < packs; i += BLOCK) grad_pack<T, N, A>(*(const Pack<T, N>*)(in + head + i * N), out, head + i * N, y, hi, c, scale, at_target);
-        for (int64_t k = lo + tid; k < head; k += BLOCK) grad_pack<T, 1, A>({{in[k]}}, out, k, y, hi, c, scale, at_target);
-        for (int64_t k = done + tid; k < hi_v; k += BLOCK) grad_pack<T, 1, A>({{in[k]}}, out, k, y, hi, c, scale, at_target);
+        for (; i < packs; i += BLOCK) grad_pack<PAST, T, N, A>(*(const Pack<T, N>*)(in + head + i * N), out, head + i * N, y, hi, c, scale, at_target);
+        for (int64_t k = lo + tid; k < head; k += BLOCK) grad_pack<PAST, T, 1, A>({{in[k]}}, out, k, y, hi, c, scale, at_target);
+        for (int64_t k = done + tid; k < hi_v; k += BLOCK) grad_pack<PAST, T, 1, A>({{in[k]}}, out, k, y, hi, c, scale, at_target);
     }
 }
 
 // ------------------------------------------------------------------------------------ launches
+// A gradient of so many bytes is stored past the caches (half of the last one's 256 MB: a smaller one may be there for whoever reads it
+// next).  Forward and gradient of other logits in every pass: 8192 x 32768 in bf16 254 us (294 through the caches), 1020 x 50001 in f32 104 (119).
+constexpr double PAST_CACHES = 128e6;
 constexpr int64_t MOST_BLOCKS = 1 << 22;  // a launch has less than 2^32 threads: kernels loop beyond
 
 static int64_t elem_size(int dtype) { return dtype == LBFGS_TRAIN_F64 ? 8 : dtype == LBFGS_TRAIN_F32 ? 4 : 2; }
@@ -287,17 +301,20 @@ static void launch_grad(const void* x, const Rows& r, double tau, const double* 
     const int64_t bytes = r.vocab * (int64_t)sizeof(T);
     // Workgroups to a row: so many that there are 512 of 16 KiB at least, or 2048 of 64 KiB.  Measured for one to a row, 512 and 2048 in all,
     // in us: in bf16 64 rows of 131072 16.6, 6.7, 9.8, 1 row 14.5, 3.2, 3.3, 255 rows of 32768 9.3, 6.9, 9.8, 1000 of 8192 6.9, 6.9, 9.8; in
-    // f32, forward and gradient, 1020 of 50001 123, 123, 117.
+    // f32, forward and gradient, 1020 of 50001 123, 123, 117 (all of them through the caches).
     auto shares = [&](int64_t all, int64_t least) { return std::min(all / r.rows, bytes / least); };
     int64_t splits = std::max<int64_t>({1, shares(512, 16384), shares(2048, 65536)});
     const int64_t part = part_of(r.vocab, (int)splits);
     splits = (r.vocab + part - 1) / part;
     const int64_t units = r.rows * splits;
     const unsigned grid = (unsigned)(units < MOST_BLOCKS ? units : MOST_BLOCKS);
-    if (bytes <= 4096)
-        logprobs_grad_kernel<T, 64><<<grid, 64, 0, s>>>((const T*)x, r, tau, c, (int)splits, part, lse, (const A*)grad, (T*)dx);
+    auto launch = [&](auto kernel, int block) { kernel<<<grid, block, 0, s>>>((const T*)x, r, tau, c, (int)splits, part, lse, (const A*)grad, (T*)dx); };
+    if (bytes <= 4096)  // (many short rows: no logits worth keeping)
+        launch(logprobs_grad_kernel<T, 64, false>, 64);
+    else if ((double)r.rows * bytes < PAST_CACHES)
+        launch(logprobs_grad_kernel<T, 256, false>, 256);
     else
-        logprobs_grad_kernel<T, 256><<<grid, 256, 0, s>>>((const T*)x, r, tau, c, (int)splits, part, lse, (const A*)grad, (T*)dx);
+        launch(logprobs_grad_kernel<T, 256, true>, 256);
 }
 
 static int check_rows(const lbfgs_train_rows* q, double temperature, Rows* r, const char* who) {
