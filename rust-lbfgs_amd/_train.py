@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import importlib.machinery
 import importlib.util
+import operator
 import os
 
 import torch  # before the library: it has to bind to torch's HIP runtime
@@ -149,6 +150,14 @@ def like(name, t, what, dtype, shape):
         raise TypeError(f"{name} is a view whose sign is still to be applied: resolve_neg() first")
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)} as {what} asks for, not {tuple(t.shape)}")
+
+
+def whole(name, v, bits):
+    """`v` as a number that the C-ABI's signed integer of so many bits holds: ctypes would keep the low bits of any other."""
+    v = operator.index(v)
+    if not -(1 << bits - 1) <= v < 1 << bits - 1:
+        raise ValueError(f"{name} must fit {bits} bits, {v} does not")
+    return v
 
 
 def ptr(t):

@@ -36,6 +36,7 @@ def orthogonalize(update, *, steps=5, coefficients=COEFFICIENTS):
         raise ValueError(f"update must be [..., rows, cols], not {tuple(update.shape)}")
     if len(coefficients) != 3:
         raise ValueError(f"coefficients are (a, b, c), not {coefficients!r}")
+    steps = _train.whole("steps", steps, 32)
     dev = _train.on_gpu("update", update)
     L = _train.load()
     g = update if update.is_contiguous() else update.detach().contiguous()

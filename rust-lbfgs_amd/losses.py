@@ -37,6 +37,7 @@ def _rows(logits, targets, ignore_index):
         raise TypeError(f"targets must be an int64 tensor, not {getattr(targets, 'dtype', type(targets).__name__)}")
     if targets.shape != logits.shape[:-1]:
         raise ValueError(f"targets must have shape {tuple(logits.shape[:-1])}, one for each row of logits, not {tuple(targets.shape)}")
+    ignore_index = _train.whole("ignore_index", ignore_index, 64)
     dev = _train.on_gpu("logits", logits, (("targets", targets),))
     if not targets.is_contiguous():
         targets = targets.contiguous()

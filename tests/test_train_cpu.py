@@ -259,6 +259,24 @@ def test_views_with_a_sign_to_come_are_refused(lib):
             call()
 
 
+@pytest.mark.parametrize("value", [1 << 70, 2 ** 64, 2 ** 64 + 5, 1 << 63, -(1 << 63) - 1, -2 ** 64 - 100])
+def test_whole_numbers_that_do_not_fit_are_refused(lib, value):
+    """Their low bits alone would be another number that is offered: 0, 5, ..."""
+    x, y = torch.zeros(2, 8), torch.zeros(2, dtype=torch.int64)
+    for call in (lambda: losses.token_logprobs(x, y, ignore_index=value), lambda: losses.token_logprobs(x.clone().requires_grad_(), y, ignore_index=value),
+                 lambda: losses.token_logprobs_with_lse(x, y, ignore_index=value), lambda: losses.token_logprobs_with_lse(torch.zeros(2, 9)[:, :8], y, ignore_index=value),
+                 lambda: losses.token_logprobs_grad(x, y, torch.zeros(2, 2, dtype=torch.float64), torch.zeros(2), ignore_index=value)):
+        with pytest.raises(ValueError, match="ignore_index must fit 64 bits"):
+            call()
+    for steps in (value, 2 ** 32 + 5, -2 ** 32 + 5, 2 ** 31):
+        with pytest.raises(ValueError, match="steps must fit 32 bits"):
+            directions.orthogonalize(torch.zeros(2, 3), steps=steps)
+    with pytest.raises(TypeError):
+        losses.token_logprobs(x, y, ignore_index=1.5)
+    with pytest.raises(TypeError):
+        directions.orthogonalize(torch.zeros(2, 3), steps=5.5)
+
+
 def test_native_calls_decline_what_is_not_ordinary(lib):
     """Tensors that are elsewhere, of other types or shapes, or no tensors at all: None, and nothing done."""
     c = _train.calls()
