@@ -13,6 +13,7 @@ import operator
 import os
 
 import torch  # before the library: it has to bind to torch's HIP runtime
+from torch.autograd import forward_ad
 
 from . import _build, _ffi
 from .api import _raise
@@ -125,8 +126,15 @@ def floating(name, t):
         raise TypeError(f"{name} must be a torch tensor, not {type(t).__name__}")
     if t.dtype not in DTYPES:
         raise TypeError(f"{name} must be float64, float32, bfloat16 or float16, not {t.dtype}")
+    plain(name, t)
+
+
+def plain(name, t):
+    """`t` is what its memory holds, and nothing else: the kernels see no more of it."""
     if t.is_neg():
         raise TypeError(f"{name} is a view whose sign is still to be applied: resolve_neg() first")
+    if forward_ad.unpack_dual(t).tangent is not None:
+        raise TypeError(f"{name} carries a forward-mode derivative, which the operators do not have: the result's would be lost")
 
 
 def on_gpu(name, t, others=()):
@@ -146,8 +154,7 @@ def like(name, t, what, dtype, shape):
         raise TypeError(f"{name} must be a torch tensor, not {type(t).__name__}")
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype} as {what} asks for, not {t.dtype}")
-    if t.is_neg():
-        raise TypeError(f"{name} is a view whose sign is still to be applied: resolve_neg() first")
+    plain(name, t)
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)} as {what} asks for, not {tuple(t.shape)}")
 

@@ -45,11 +45,13 @@ int type_of(at::ScalarType t) {
 }
 at::ScalarType wide(at::ScalarType t) { return t == at::kDouble ? at::kDouble : at::kFloat; }
 
-// a tensor as the kernels want it, or NULL: dense, plain (no subclass that has a say in what happens to it), with its sign applied
+// a tensor as the kernels want it, or NULL: dense, plain (no subclass that has a say in what happens to it), with its sign applied and
+// without a forward-mode derivative
 const at::Tensor* tensor(PyObject* o) {
     if (!THPVariable_Check(o)) return nullptr;
     const at::Tensor& t = THPVariable_Unpack(o);
-    if (!t.defined() || t.layout() != at::kStrided || !t.is_cuda() || !t.is_contiguous() || t.is_neg() || t.key_set().has(c10::DispatchKey::Python)) return nullptr;
+    if (!t.defined() || t.layout() != at::kStrided || !t.is_cuda() || !t.is_contiguous() || t.is_neg() || t.key_set().has(c10::DispatchKey::Python) || t._fw_grad(0).defined())
+        return nullptr;
     return &t;
 }
 const at::Tensor* floating(PyObject* o) {

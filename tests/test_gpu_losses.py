@@ -654,6 +654,28 @@ def test_tensors_on_different_devices_are_refused():
         losses.token_logprobs(lp, torch.zeros(2, dtype=torch.int64))
 
 
+def test_forward_mode_derivatives_are_refused():
+    """Dense plain tensors of the GPU, which the native calls would take, with a tangent that the result would not have."""
+    from torch.autograd import forward_ad
+
+    from rust_lbfgs_amd import directions
+
+    x, y, g = make((3, 4), 50, torch.float32)
+    lp = -torch.rand(4, 5).cuda()
+    A = torch.ones(4, 1).cuda()
+    _, lse = losses.token_logprobs_with_lse(x, y)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: losses.token_logprobs(dual(x), y), lambda: losses.token_logprobs(dual(x)[:, 1:], y[:, 1:]), lambda: losses.token_logprobs_with_lse(dual(x), y),
+                     lambda: losses.token_logprobs_grad(dual(x), y, lse, g), lambda: losses.token_logprobs_grad(x, y, dual(lse), g),
+                     lambda: losses.token_logprobs_grad(x, y, lse, dual(g)), lambda: losses.preference(dual(lp)), lambda: losses.preference_loss(lp, dual(lp)),
+                     lambda: losses.policy(dual(lp), lp, lp), lambda: losses.policy_loss(lp, dual(lp), lp), lambda: losses.policy(lp, lp, dual(A)),
+                     lambda: losses.policy(lp, lp, lp, ref_logps=dual(lp), kl_coef=0.1), lambda: directions.orthogonalize(dual(x[0]))):
+            with pytest.raises(TypeError, match="forward-mode derivative"):
+                call()
+        assert losses.preference(lp).f.isfinite()  # a level alone takes nothing away
+
+
 @pytest.mark.parametrize("bad", [dict(beta=-1.0), dict(label_smoothing=0.7), dict(label_smoothing=0.1, kind="hinge")])
 def test_refused_calls_raise_and_leave_the_next_one_alone(bad):
     lp = -torch.rand(4, 5).cuda()

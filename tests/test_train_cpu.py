@@ -277,6 +277,22 @@ def test_whole_numbers_that_do_not_fit_are_refused(lib, value):
         directions.orthogonalize(torch.zeros(2, 3), steps=5.5)
 
 
+def test_forward_mode_derivatives_are_refused(lib):
+    """A dual tensor has requires_grad False: taken as it is, its tangent would be lost and read as a derivative of 0."""
+    from torch.autograd import forward_ad
+
+    x, y, off = torch.zeros(6), torch.zeros((), dtype=torch.int64), torch.tensor([0, 2, 6])
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones(6))
+        view = d.view(2, 3)
+        for call in (lambda: losses.token_logprobs(d, y), lambda: losses.token_logprobs_with_lse(d, y), lambda: losses.token_logprobs_grad(d, y, x, x),
+                     lambda: losses.preference(d, offsets=off), lambda: losses.preference_loss(view), lambda: losses.preference_loss(x, d, offsets=off),
+                     lambda: losses.policy_loss(d, x, x, offsets=off), lambda: losses.policy(x, d, x, offsets=off), lambda: losses.policy(x, x, d, offsets=off),
+                     lambda: losses.policy(x, x, x, ref_logps=d, kl_coef=0.1, offsets=off), lambda: directions.orthogonalize(view)):
+            with pytest.raises(TypeError, match="forward-mode derivative"):
+                call()
+
+
 def test_native_calls_decline_what_is_not_ordinary(lib):
     """Tensors that are elsewhere, of other types or shapes, or no tensors at all: None, and nothing done."""
     c = _train.calls()
