@@ -71,11 +71,14 @@ int lbfgs_train_token_logprobs_grad(const lbfgs_train_rows* rows, double tempera
  * decreasing, 32 or 64 bits), or, with offsets NULL, the s-th of `count` equal parts: a padded batch.  Tokens that no
  * sequence has, and those whose mask is 0, are not looked at: their values may be anything, their gradient is 0.  Offsets that
  * decrease or leave [0, tokens] make the loss NaN (nothing out of range is read or written). */
+/* (A loss that is a mean has slopes of 1 / tokens or 1 / (pairs * length), and what is multiplied into them comes later.  By then F16, whose
+ * smallest normal number is 6e-5 and whose smallest step 6e-8, has lost bits from some 10^4 tokens on, and from 3e7 on everything.) */
+enum { LBFGS_TRAIN_WIDE_GRAD = 256 };
 typedef struct lbfgs_train_sequences {
     const void* offsets;
     const uint8_t* mask;       /* [tokens] or NULL */
     int32_t offset_bits;
-    int32_t dtype;             /* of every tensor over tokens */
+    int32_t dtype;             /* of every tensor over tokens; | LBFGS_TRAIN_WIDE_GRAD: but of grad, which is in the wide type */
     int64_t tokens, count;
 } lbfgs_train_sequences;
 uint64_t lbfgs_train_sequences_workspace(int64_t tokens, int64_t count);

@@ -20,6 +20,7 @@ from .api import _raise
 
 ABI_VERSION = 1  # LBFGS_TRAIN_ABI_VERSION of the header these declarations were written against
 DTYPES = {torch.float64: 0, torch.float32: 1, torch.bfloat16: 2, torch.float16: 3}
+WIDE_GRAD = 256  # LBFGS_TRAIN_WIDE_GRAD
 
 
 class Rows(C.Structure):

@@ -222,7 +222,9 @@ bool another(PyObject* o, const at::Tensor& x, const at::Tensor** t) {
 }
 const void* data(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
 
-// preference(logps, ref_logps, offsets, mask, beta, label_smoothing, kind, normalize_lengths) -> (f, rewards, grad)
+// preference(logps, ref_logps, offsets, mask, beta, label_smoothing, kind, normalize_lengths) -> (f, rewards, grad); WIDE: the gradient in
+// the wide type
+template <bool WIDE>
 PyObject* preference(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!arguments(n, 8)) return nullptr;
     return guarded([&]() -> PyObject* {
@@ -235,7 +237,8 @@ PyObject* preference(PyObject*, PyObject* const* a, Py_ssize_t n) {
             !stream_of(*x, &s))
             Py_RETURN_NONE;
         const bool normalize = a[7] == Py_True;
-        at::Tensor f = make(*x, {}, wide(x->scalar_type())), rewards = make(*x, {q.count}, wide(x->scalar_type())), grad = make(*x, x->sizes(), x->scalar_type());
+        at::Tensor f = make(*x, {}, wide(x->scalar_type())), rewards = make(*x, {q.count}, wide(x->scalar_type())), grad = make(*x, x->sizes(), WIDE ? wide(x->scalar_type()) : x->scalar_type());
+        if (WIDE) q.dtype |= LBFGS_TRAIN_WIDE_GRAD;
         const Workspace w(*x, L.sequences_workspace(q.tokens, q.count));
         const int rc = without_lock([&] {
             return L.preference(&q, x->data_ptr(), data(ref), beta, smoothing, (int32_t)kind, normalize, f.data_ptr(), rewards.data_ptr(), grad.data_ptr(), w.data, w.bytes, s);
@@ -244,6 +247,7 @@ PyObject* preference(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 // policy(logps, old_logps, advantages, ref_logps, offsets, mask, clip_low, clip_high, kl_coef, by_sequence) -> (f, kl, clip_fraction, grad)
+template <bool WIDE>
 PyObject* policy(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!arguments(n, 10)) return nullptr;
     return guarded([&]() -> PyObject* {
@@ -259,7 +263,8 @@ PyObject* policy(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const bool per_token = !(adv && adv->sizes() == at::IntArrayRef(each, 2));
         if (!like(adv, *x, x->scalar_type(), per_token ? x->sizes() : at::IntArrayRef(each, 2)) || (kl_coef != 0 && !ref) || !stream_of(*x, &s)) Py_RETURN_NONE;
         const at::ScalarType out = wide(x->scalar_type());
-        at::Tensor f = make(*x, {}, out), kl = make(*x, {}, out), clipped = make(*x, {}, out), grad = make(*x, x->sizes(), x->scalar_type());
+        at::Tensor f = make(*x, {}, out), kl = make(*x, {}, out), clipped = make(*x, {}, out), grad = make(*x, x->sizes(), WIDE ? out : x->scalar_type());
+        if (WIDE) q.dtype |= LBFGS_TRAIN_WIDE_GRAD;
         const Workspace w(*x, L.sequences_workspace(q.tokens, q.count));
         const int rc = without_lock([&] {
             return L.policy(&q, x->data_ptr(), old->data_ptr(), data(ref), adv->data_ptr(), per_token, low, high, kl_coef, (int32_t)by_sequence, f.data_ptr(), kl.data_ptr(),
@@ -303,8 +308,10 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_NONE;
 }
 
-#define METHOD(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {METHOD(bind), METHOD(logprobs), METHOD(logprobs_grad), METHOD(preference), METHOD(policy), METHOD(orthogonalize), {nullptr, nullptr, 0, nullptr}};
+#define METHOD(name, ...) {#name, (PyCFunction)(void (*)(void))__VA_ARGS__, METH_FASTCALL, nullptr}
+PyMethodDef methods[] = {METHOD(bind, bind), METHOD(logprobs, logprobs), METHOD(logprobs_grad, logprobs_grad), METHOD(preference, preference<false>),
+                         METHOD(preference_wide, preference<true>), METHOD(policy, policy<false>), METHOD(policy_wide, policy<true>),
+                         METHOD(orthogonalize, orthogonalize), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "liblbfgs_train_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

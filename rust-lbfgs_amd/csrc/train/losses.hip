@@ -377,16 +377,16 @@ __device__ __forceinline__ void pair_losses(const Q& q, const Preference& o, con
 
 // gradient of chunk w: its sequence's slope at each token that counts, 0 at all others.  slope[(s - base) & within]: with a table of
 // the chunk's own sequences, bad offsets still lead nowhere else.
-template <class T, class Q>
-__device__ __forceinline__ void chunk_slopes(const Q& q, const double* slope, int64_t base, int64_t within, T* grad, int64_t w, Spot at, const Pack<uint8_t, E>& keep) {
-    typedef typename Num<T>::acc A;
+template <class G, class Q>
+__device__ __forceinline__ void chunk_slopes(const Q& q, const double* slope, int64_t base, int64_t within, G* grad, int64_t w, Spot at, const Pack<uint8_t, E>& keep) {
+    typedef typename Num<G>::acc A;
     const int64_t t0 = w * CHUNK + threadIdx.x * E;
     if (t0 >= q.tokens) return;
-    Pack<T, E> g;
+    Pack<G, E> g;
     A v = at.s < q.count ? (A)slope[(at.s - base) & within] : 0;
 #pragma unroll
     for (int k = 0; k < E; k++) {
-        g.v[k] = k >= at.begin && k < at.end && keep.v[k] ? (T)v : (T)0;
+        g.v[k] = k >= at.begin && k < at.end && keep.v[k] ? (G)v : (G)0;
         if (k + 1 == at.end) {
             q.next(at, t0);
             if (k + 1 < E) v = at.s < q.count ? (A)slope[(at.s - base) & within] : 0;
@@ -415,8 +415,8 @@ template <int GROUP, class A>
 __global__ __launch_bounds__(BLOCK) void pairs_kernel(Seqs q, Preference o, Space sp, A* rewards) {
     pair_losses<GROUP>(q, o, sp, rewards, true, blockIdx.x, gridDim.x);
 }
-template <class T>
-__global__ __launch_bounds__(BLOCK) void slopes_kernel(Seqs q, int64_t chunks, int blocks, Space sp, typename Num<T>::acc* f, T* grad) {
+template <class G>
+__global__ __launch_bounds__(BLOCK) void slopes_kernel(Seqs q, int64_t chunks, int blocks, Space sp, typename Num<G>::acc* f, G* grad) {
     if (blockIdx.x == 0) mean_loss(sp, blocks, q.count / 2, f);
     for (int64_t w = blockIdx.x; w < chunks; w += gridDim.x) {
         const int64_t t0 = w * CHUNK + threadIdx.x * E;
@@ -429,13 +429,13 @@ __global__ __launch_bounds__(BLOCK) void slopes_kernel(Seqs q, int64_t chunks, i
 // their partners'; the last workgroup, which has no chunk, the loss and the rewards.
 constexpr int64_t FEW_SEQS = 1024;  // (a power of two)
 constexpr int64_t FEW_LONG_SEQS = 128;  // ... of many chunks (in us: 128 of 20000 16.9, 17.9; 256 of 20000 27.6, 24.9; 1000 of 8200 63, 32)
-template <class T, int GROUP>
-__global__ __launch_bounds__(BLOCK) void few_slopes_kernel(Seqs q, Preference o, int64_t chunks, Space sp, typename Num<T>::acc* f, typename Num<T>::acc* rewards, T* grad) {
+template <class G, int GROUP>
+__global__ __launch_bounds__(BLOCK) void few_slopes_kernel(Seqs q, Preference o, int64_t chunks, Space sp, typename Num<G>::acc* f, typename Num<G>::acc* rewards, G* grad) {
     __shared__ double slope[FEW_SEQS];
     __shared__ int64_t ends[2];
     if (blockIdx.x == gridDim.x - 1) {
         pair_losses<GROUP>(q, o, sp, rewards, false, 0, 1);
-        if (threadIdx.x == 0) *f = (typename Num<T>::acc)(sp.loss[0] / (double)(q.count / 2));
+        if (threadIdx.x == 0) *f = (typename Num<G>::acc)(sp.loss[0] / (double)(q.count / 2));
         return;
     }
     const int64_t pairs = q.count / 2, groups = gridDim.x - 1;
@@ -474,9 +474,9 @@ __global__ __launch_bounds__(BLOCK) void few_slopes_kernel(Seqs q, Preference o,
     }
 }
 // a small batch: all of it as one workgroup, with nothing between the passes but LDS
-template <class T>
+template <class T, class G>
 __global__ __launch_bounds__(BLOCK) void preference_small_kernel(Seqs whole, Preference o, const T* a, const T* b, int chunks,
-                                                                 typename Num<T>::acc* f, typename Num<T>::acc* rewards, T* grad) {
+                                                                 typename Num<T>::acc* f, typename Num<T>::acc* rewards, G* grad) {
     __shared__ SmallSpace m;
     Space sp;
     Tokens<T> x[SMALL_CHUNKS];
@@ -629,17 +629,18 @@ __device__ __forceinline__ void ratio(const Policy& o, double lp, double old, do
     ra = a == 0 && d == d ? 0 : exp(d) * a;
 }
 
-template <class T>
+template <class T, class G>
 struct PolicyData {
     const T *logps, *old, *ref, *adv;
-    T* grad;
+    G* grad;
 };
 // a thread's tokens
 template <class T>
 struct PolicyTokens {
     Pack<T, E> lp, old, ref, adv;
     Pack<uint8_t, E> keep;
-    __device__ __forceinline__ void get(const PolicyData<T>& x, const uint8_t* mask, bool per_token, int64_t t, int64_t n) {
+    template <class G>
+    __device__ __forceinline__ void get(const PolicyData<T, G>& x, const uint8_t* mask, bool per_token, int64_t t, int64_t n) {
         load(x.logps, t, n, lp);
         load(x.old, t, n, old);
         if (x.ref) load(x.ref, t, n, ref);
@@ -671,13 +672,13 @@ __device__ __forceinline__ void token(const Policy& o, T lp, T old, T ref, doubl
     slope *= weight;
 }
 
-template <class T, class Q>
-__device__ __forceinline__ void chunk_policy(const Q& q, const Policy& o, const PolicyTokens<T>& x, const T* advantages, T* grad, const double* inverse, double inv,
+template <class T, class G, class Q>
+__device__ __forceinline__ void chunk_policy(const Q& q, const Policy& o, const PolicyTokens<T>& x, const T* advantages, G* grad, const double* inverse, double inv,
                                              int64_t w, double& f, double& kl, double& clipped) {
     const int64_t t0 = w * CHUNK + threadIdx.x * E, n = q.tokens;
     Spot at = q.locate(t0);
     if (t0 >= n) return;
-    Pack<T, E> g;
+    Pack<G, E> g;
     double a_seq = 0, weight = inv;
     auto enter = [&]() {
         if (at.s < q.count) {
@@ -691,7 +692,7 @@ __device__ __forceinline__ void chunk_policy(const Q& q, const Policy& o, const 
         double slope = 0;
         if (k >= at.begin && k < at.end && x.keep.v[k])
             token<T>(o, x.lp.v[k], x.old.v[k], x.ref.v[k], o.per_token ? (double)x.adv.v[k] : a_seq, weight, slope, f, kl, clipped);
-        g.v[k] = (T)slope;
+        g.v[k] = (G)slope;
         if (k + 1 == at.end) {
             q.next(at, t0);
             if (k + 1 < E) enter();
@@ -709,8 +710,8 @@ __device__ __forceinline__ void policy_results(double f, double kl, double clipp
 }
 
 __global__ __launch_bounds__(BLOCK) void weights_kernel(Seqs q, Space sp) { sequence_weights(q, sp, blockIdx.x, gridDim.x); }
-template <class T>
-__global__ __launch_bounds__(BLOCK) void policy_kernel(Seqs q, Policy o, PolicyData<T> x, int64_t chunks, int count_blocks, Space sp) {
+template <class T, class G>
+__global__ __launch_bounds__(BLOCK) void policy_kernel(Seqs q, Policy o, PolicyData<T, G> x, int64_t chunks, int count_blocks, Space sp) {
     double kept, some, f = 0, kl = 0, clipped = 0;
     all_counts(sp, count_blocks, kept, some);
     const double inv = 1.0 / (o.by_sequence ? some : kept);
@@ -728,15 +729,16 @@ __global__ __launch_bounds__(BLOCK) void policy_kernel(Seqs q, Policy o, PolicyD
 // alike, and nobody looks for their sequences.  One pack of 16 bytes of each tensor a thread.  2048 x 4096 tokens in 32 bits with a
 // reference: 30.1 us in all (36.3 by the pass that knows sequences).
 constexpr int ALIKE_BLOCKS = 1280;  // five to a compute unit
-template <class T>
-__global__ __launch_bounds__(BLOCK) void policy_alike_kernel(Seqs q, Policy o, PolicyData<T> x, int count_blocks, Space sp) {
+template <class T, class G>
+__global__ __launch_bounds__(BLOCK) void policy_alike_kernel(Seqs q, Policy o, PolicyData<T, G> x, int count_blocks, Space sp) {
     constexpr int N = vec_len<T>();
     double kept, some, f = 0, kl = 0, clipped = 0;
     all_counts(sp, count_blocks, kept, some);
     const double inv = 1.0 / kept;
     const int64_t begin = q.at(0), end = q.at(q.count), n = q.tokens, stride = (int64_t)gridDim.x * BLOCK * N;
     for (int64_t t = ((int64_t)blockIdx.x * BLOCK + threadIdx.x) * N; t < n; t += stride) {
-        Pack<T, N> lp, old, ref, adv, g;
+        Pack<T, N> lp, old, ref, adv;
+        Pack<G, N> g;
         Pack<uint8_t, N> keep;
         if (t + N <= n) {
             lp = *(const Pack<T, N>*)(x.logps + t), old = *(const Pack<T, N>*)(x.old + t), adv = *(const Pack<T, N>*)(x.adv + t);
@@ -746,15 +748,15 @@ __global__ __launch_bounds__(BLOCK) void policy_alike_kernel(Seqs q, Policy o, P
             for (int k = 0; k < N; k++) {
                 double slope = 0;
                 if (t + k >= begin && t + k < end && (!q.mask || keep.v[k])) token<T>(o, lp.v[k], old.v[k], ref.v[k], (double)adv.v[k], 1.0, slope, f, kl, clipped);
-                g.v[k] = (T)(slope * inv);
+                g.v[k] = (G)(slope * inv);
             }
-            *(Pack<T, N>*)(x.grad + t) = g;
+            *(Pack<G, N>*)(x.grad + t) = g;
         } else {
             for (int64_t k = t; k < n; k++) {
                 double slope = 0;
                 if (k >= begin && k < end && (!q.mask || q.mask[k]))
                     token<T>(o, x.logps[k], x.old[k], x.ref ? x.ref[k] : (T)0, (double)x.adv[k], 1.0, slope, f, kl, clipped);
-                x.grad[k] = (T)(slope * inv);
+                x.grad[k] = (G)(slope * inv);
             }
         }
     }
@@ -770,8 +772,8 @@ __global__ __launch_bounds__(BLOCK) void policy_results_kernel(Space sp, int cou
     for (int k = threadIdx.x; k < blocks; k += BLOCK) f += sp.sums[3 * k], kl += sp.sums[3 * k + 1], clipped += sp.sums[3 * k + 2];
     policy_results(f, kl, clipped, kept, out_f, out_kl, out_clipped);
 }
-template <class T>
-__global__ __launch_bounds__(BLOCK) void policy_small_kernel(Seqs whole, Policy o, PolicyData<T> x, int chunks, typename Num<T>::acc* out_f,
+template <class T, class G>
+__global__ __launch_bounds__(BLOCK) void policy_small_kernel(Seqs whole, Policy o, PolicyData<T, G> x, int chunks, typename Num<T>::acc* out_f,
                                                              typename Num<T>::acc* out_kl, typename Num<T>::acc* out_clipped) {
     __shared__ SmallSpace m;
     Space sp;
@@ -845,12 +847,12 @@ static uint64_t lay_out(Space* sp, void* base, int64_t tokens, int64_t seqs) {
     return at;
 }
 
-template <class T>
+template <class T, class G>
 static void launch_preference(const Seqs& q, const Preference& o, const void* a, const void* b, void* f, void* rewards, void* grad, const Space& sp, hipStream_t s) {
     typedef typename Num<T>::acc A;
     const int64_t chunks = chunks_of(q.tokens), pairs = q.count / 2;
     if (small(q.tokens, q.count)) {
-        preference_small_kernel<T><<<1, BLOCK, 0, s>>>(q, o, (const T*)a, (const T*)b, (int)chunks, (A*)f, (A*)rewards, (T*)grad);
+        preference_small_kernel<T, G><<<1, BLOCK, 0, s>>>(q, o, (const T*)a, (const T*)b, (int)chunks, (A*)f, (A*)rewards, (G*)grad);
         return;
     }
     // The records of a sequence (one for each chunk it reaches) are added up by one lane, or by eight where there are many.  Measured, in
@@ -863,26 +865,26 @@ static void launch_preference(const Seqs& q, const Preference& o, const void* a,
     if (q.count <= (many ? FEW_LONG_SEQS : FEW_SEQS)) {
         const unsigned grid = (unsigned)(chunks < 768 ? chunks : 768);  // (three to a compute unit: all of them at once)
         if (many)
-            few_slopes_kernel<T, 8><<<grid + 1, BLOCK, 0, s>>>(q, o, chunks, sp, (A*)f, (A*)rewards, (T*)grad);
+            few_slopes_kernel<G, 8><<<grid + 1, BLOCK, 0, s>>>(q, o, chunks, sp, (A*)f, (A*)rewards, (G*)grad);
         else
-            few_slopes_kernel<T, 1><<<grid + 1, BLOCK, 0, s>>>(q, o, chunks, sp, (A*)f, (A*)rewards, (T*)grad);
+            few_slopes_kernel<G, 1><<<grid + 1, BLOCK, 0, s>>>(q, o, chunks, sp, (A*)f, (A*)rewards, (G*)grad);
         return;
     }
     if (many)
         pairs_kernel<8, A><<<blocks, BLOCK, 0, s>>>(q, o, sp, (A*)rewards);
     else
         pairs_kernel<1, A><<<blocks, BLOCK, 0, s>>>(q, o, sp, (A*)rewards);
-    slopes_kernel<T><<<grid, BLOCK, 0, s>>>(q, chunks, blocks, sp, (A*)f, (T*)grad);
+    slopes_kernel<G><<<grid, BLOCK, 0, s>>>(q, chunks, blocks, sp, (A*)f, (G*)grad);
 }
 
-template <class T>
+template <class T, class G>
 static void launch_policy(const Seqs& q, const Policy& o, const void* logps, const void* old, const void* ref, const void* adv, void* f, void* kl,
                           void* clipped, void* grad, const Space& sp, hipStream_t s) {
     typedef typename Num<T>::acc A;
     const int64_t chunks = chunks_of(q.tokens);
-    const PolicyData<T> x = {(const T*)logps, (const T*)old, (const T*)ref, (const T*)adv, (T*)grad};
+    const PolicyData<T, G> x = {(const T*)logps, (const T*)old, (const T*)ref, (const T*)adv, (G*)grad};
     if (small(q.tokens, q.count)) {
-        policy_small_kernel<T><<<1, BLOCK, 0, s>>>(q, o, x, (int)chunks, (A*)f, (A*)kl, (A*)clipped);
+        policy_small_kernel<T, G><<<1, BLOCK, 0, s>>>(q, o, x, (int)chunks, (A*)f, (A*)kl, (A*)clipped);
         return;
     }
     const bool total = q.mask && !o.by_sequence;  // the number of all tokens is wanted, not each sequence's
@@ -898,16 +900,17 @@ static void launch_policy(const Seqs& q, const Policy& o, const void* logps, con
     if (o.per_token && !o.by_sequence) {
         const int64_t packs = (q.tokens + vec_len<T>() - 1) / vec_len<T>(), need = (packs + BLOCK - 1) / BLOCK;
         blocks = (int)(need < ALIKE_BLOCKS ? (need ? need : 1) : ALIKE_BLOCKS);
-        policy_alike_kernel<T><<<blocks, BLOCK, 0, s>>>(q, o, x, count_blocks, sp);
+        policy_alike_kernel<T, G><<<blocks, BLOCK, 0, s>>>(q, o, x, count_blocks, sp);
     } else {
-        policy_kernel<T><<<blocks, BLOCK, 0, s>>>(q, o, x, chunks, count_blocks, sp);
+        policy_kernel<T, G><<<blocks, BLOCK, 0, s>>>(q, o, x, chunks, count_blocks, sp);
     }
     policy_results_kernel<A><<<1, BLOCK, 0, s>>>(sp, count_blocks, blocks, (A*)f, (A*)kl, (A*)clipped);
 }
 
 static int check_seqs(const lbfgs_train_sequences* in, Seqs* q, const char* who) {
     if (!in) return lt_fail(LBFGS_HIP_ERR_ARG, "%s: no sequences", who);
-    if (in->dtype < LBFGS_TRAIN_F64 || in->dtype > LBFGS_TRAIN_F16) return lt_fail(LBFGS_HIP_ERR_ARG, "%s: unknown element type %d", who, in->dtype);
+    if ((in->dtype & ~LBFGS_TRAIN_WIDE_GRAD) < LBFGS_TRAIN_F64 || (in->dtype & ~LBFGS_TRAIN_WIDE_GRAD) > LBFGS_TRAIN_F16)
+        return lt_fail(LBFGS_HIP_ERR_ARG, "%s: unknown element type %d", who, in->dtype);
     if (in->tokens < 0 || in->count < 1 || in->tokens > (INT64_MAX >> 20) || in->count > (INT64_MAX >> 20))
         return lt_fail(LBFGS_HIP_ERR_ARG, "%s: %lld tokens in %lld sequences", who, (long long)in->tokens, (long long)in->count);
     if (in->offsets) {
@@ -980,10 +983,14 @@ extern "C" int lbfgs_train_preference(const lbfgs_train_sequences* seqs, const v
     const Preference o = {beta, label_smoothing, kind, normalize_lengths != 0};
     hipStream_t s = (hipStream_t)stream;
     switch (seqs->dtype) {
-        case LBFGS_TRAIN_F64: launch_preference<double>(q, o, logps, ref_logps, f, rewards, grad, sp, s); break;
-        case LBFGS_TRAIN_F32: launch_preference<float>(q, o, logps, ref_logps, f, rewards, grad, sp, s); break;
-        case LBFGS_TRAIN_BF16: launch_preference<bf16>(q, o, logps, ref_logps, f, rewards, grad, sp, s); break;
-        default: launch_preference<f16>(q, o, logps, ref_logps, f, rewards, grad, sp, s);
+        case LBFGS_TRAIN_F64:
+        case LBFGS_TRAIN_F64 | LBFGS_TRAIN_WIDE_GRAD: launch_preference<double, double>(q, o, logps, ref_logps, f, rewards, grad, sp, s); break;
+        case LBFGS_TRAIN_F32:
+        case LBFGS_TRAIN_F32 | LBFGS_TRAIN_WIDE_GRAD: launch_preference<float, float>(q, o, logps, ref_logps, f, rewards, grad, sp, s); break;
+        case LBFGS_TRAIN_BF16: launch_preference<bf16, bf16>(q, o, logps, ref_logps, f, rewards, grad, sp, s); break;
+        case LBFGS_TRAIN_F16: launch_preference<f16, f16>(q, o, logps, ref_logps, f, rewards, grad, sp, s); break;
+        case LBFGS_TRAIN_BF16 | LBFGS_TRAIN_WIDE_GRAD: launch_preference<bf16, float>(q, o, logps, ref_logps, f, rewards, grad, sp, s); break;
+        default: launch_preference<f16, float>(q, o, logps, ref_logps, f, rewards, grad, sp, s);
     }
     return lt_launched(who);
 }
@@ -1006,10 +1013,14 @@ extern "C" int lbfgs_train_policy(const lbfgs_train_sequences* seqs, const void*
     if (kl_coef == 0) ref_logps = nullptr;
     hipStream_t s = (hipStream_t)stream;
     switch (seqs->dtype) {
-        case LBFGS_TRAIN_F64: launch_policy<double>(q, o, logps, old_logps, ref_logps, advantages, f, kl, clip_fraction, grad, sp, s); break;
-        case LBFGS_TRAIN_F32: launch_policy<float>(q, o, logps, old_logps, ref_logps, advantages, f, kl, clip_fraction, grad, sp, s); break;
-        case LBFGS_TRAIN_BF16: launch_policy<bf16>(q, o, logps, old_logps, ref_logps, advantages, f, kl, clip_fraction, grad, sp, s); break;
-        default: launch_policy<f16>(q, o, logps, old_logps, ref_logps, advantages, f, kl, clip_fraction, grad, sp, s);
+        case LBFGS_TRAIN_F64:
+        case LBFGS_TRAIN_F64 | LBFGS_TRAIN_WIDE_GRAD: launch_policy<double, double>(q, o, logps, old_logps, ref_logps, advantages, f, kl, clip_fraction, grad, sp, s); break;
+        case LBFGS_TRAIN_F32:
+        case LBFGS_TRAIN_F32 | LBFGS_TRAIN_WIDE_GRAD: launch_policy<float, float>(q, o, logps, old_logps, ref_logps, advantages, f, kl, clip_fraction, grad, sp, s); break;
+        case LBFGS_TRAIN_BF16: launch_policy<bf16, bf16>(q, o, logps, old_logps, ref_logps, advantages, f, kl, clip_fraction, grad, sp, s); break;
+        case LBFGS_TRAIN_F16: launch_policy<f16, f16>(q, o, logps, old_logps, ref_logps, advantages, f, kl, clip_fraction, grad, sp, s); break;
+        case LBFGS_TRAIN_BF16 | LBFGS_TRAIN_WIDE_GRAD: launch_policy<bf16, float>(q, o, logps, old_logps, ref_logps, advantages, f, kl, clip_fraction, grad, sp, s); break;
+        default: launch_policy<f16, float>(q, o, logps, old_logps, ref_logps, advantages, f, kl, clip_fraction, grad, sp, s);
     }
     return lt_launched(who);
 }

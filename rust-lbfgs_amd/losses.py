@@ -130,7 +130,7 @@ def _dense(t):
     return t if t is None or t.is_contiguous() else t.detach().contiguous()
 
 
-def _sequences(logps, offsets, mask, others):
+def _sequences(logps, offsets, mask, others, wide_grad):
     """-> (Sequences, number of them, the tensors, dense, in the order logps, mask, offsets, others)."""
     _train.floating("logps", logps)
     shape, dtype = logps.shape, logps.dtype
@@ -152,7 +152,7 @@ def _sequences(logps, offsets, mask, others):
             raise ValueError(f"with offsets logps must be one-dimensional, not {tuple(shape)}")
         count, bits = offsets.shape[0] - 1, 32 if offsets.dtype == torch.int32 else 64
     x, m, o = _dense(logps), _dense(mask), _dense(offsets)
-    q = _train.Sequences(_train.ptr(o), _train.ptr(m), bits, _train.DTYPES[dtype], x.numel(), count)
+    q = _train.Sequences(_train.ptr(o), _train.ptr(m), bits, _train.DTYPES[dtype] | (_train.WIDE_GRAD if wide_grad else 0), x.numel(), count)
     return q, count, (x, m, o, *[_dense(t) for _, t in others])
 
 
@@ -162,25 +162,28 @@ class Preference(NamedTuple):
     grad: torch.Tensor      # df/dlogps
 
 
-def preference(logps, ref_logps=None, *, offsets=None, mask=None, beta=0.1, kind="logistic", label_smoothing=0.0, normalize_lengths=False):
+def preference(logps, ref_logps=None, *, offsets=None, mask=None, beta=0.1, kind="logistic", label_smoothing=0.0, normalize_lengths=False, wide_grad=False):
     """Loss of paired log ratios, value and gradient.
 
     2 P sequences: i is preferred to i + P.  With R the sum over a sequence's tokens of logps - ref_logps (ref_logps None:
     of logps; normalize_lengths: divided by their number) and h = beta (R_i - R_{i+P}), the loss of a pair is
         logistic  -(1 - label_smoothing) log sigmoid(h) - label_smoothing log sigmoid(-h)
         hinge     max(0, 1 - h)                  squared   (h / beta - 1 / (2 beta))^2
-    All sums are taken in 64 bits.  -> Preference(f, rewards, grad); f and rewards in float64 for float64 data, else float32."""
+    All sums are taken in 64 bits.  -> Preference(f, rewards, grad); f and rewards in float64 for float64 data, else float32.
+    The gradient is in the type of logps.  In 16 bits that rounds slopes of 1/pairs and 1/length before anything is multiplied into them,
+    and float16 has fewer bits for them below 6e-5 and none below 6e-8: wide_grad gives them in float32."""
     if kind not in KINDS:
         raise ValueError(f"kind must be one of {', '.join(KINDS)}, not {kind!r}")
-    done = _train.calls().preference(logps, ref_logps, offsets, mask, beta, label_smoothing, KINDS[kind], normalize_lengths)
+    calls = _train.calls()
+    done = (calls.preference_wide if wide_grad else calls.preference)(logps, ref_logps, offsets, mask, beta, label_smoothing, KINDS[kind], normalize_lengths)
     if done is not None:
         return Preference._make(_train.results(done))
     others = (("ref_logps", ref_logps),)
-    q, count, (x, m, o, ref) = _sequences(logps, offsets, mask, others)
+    q, count, (x, m, o, ref) = _sequences(logps, offsets, mask, others, wide_grad)
     dev = _train.on_gpu("logps", logps, (("offsets", offsets), ("mask", mask), *others))
     L, out = _train.load(), _train.wide(x.dtype)
     f, rewards = x.new_empty((), dtype=out), x.new_empty(count, dtype=out)
-    grad = torch.empty_like(x)
+    grad = torch.empty_like(x, dtype=out if wide_grad else x.dtype)
     size = L.lbfgs_train_sequences_workspace(q.tokens, count)
     ws = x.new_empty(size, dtype=torch.uint8) if size else None
     _train.enqueue(L.lbfgs_train_preference, dev, C.byref(q), x.data_ptr(), _train.ptr(ref), beta, label_smoothing, KINDS[kind], bool(normalize_lengths),
@@ -195,28 +198,31 @@ class Policy(NamedTuple):
     grad: torch.Tensor           # df/dlogps
 
 
-def policy(logps, old_logps, advantages, *, ref_logps=None, offsets=None, mask=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0, reduction="tokens"):
+def policy(logps, old_logps, advantages, *, ref_logps=None, offsets=None, mask=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0, reduction="tokens",
+           wide_grad=False):
     """Clipped policy loss with a KL term, value and gradient.
 
     With r = exp(logps - old_logps), q = ref_logps - logps and a token's advantage A (advantages like logps, or [S, 1]: one for
     each sequence), a token's loss is -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(q) - 1 - q); f is the
     mean over all tokens ("tokens"), or over the sequences that have any of their own means ("sequences").  clip_high may be
-    infinite.  -> Policy(f, kl, clip_fraction, grad); the scalars in float64 for float64 data, else float32."""
+    infinite.  -> Policy(f, kl, clip_fraction, grad); the scalars in float64 for float64 data, else float32.  The gradient is in the
+    type of logps; wide_grad as in preference: in float16 slopes of 1/tokens lose bits from some 10^4 tokens on."""
     if reduction not in REDUCTIONS:
         raise ValueError(f"reduction must be one of {', '.join(REDUCTIONS)}, not {reduction!r}")
     if kl_coef != 0 and ref_logps is None:
         raise ValueError("a KL term needs ref_logps")
-    done = _train.calls().policy(logps, old_logps, advantages, ref_logps, offsets, mask, clip_low, clip_high, kl_coef, REDUCTIONS[reduction])
+    calls = _train.calls()
+    done = (calls.policy_wide if wide_grad else calls.policy)(logps, old_logps, advantages, ref_logps, offsets, mask, clip_low, clip_high, kl_coef, REDUCTIONS[reduction])
     if done is not None:
         return Policy._make(_train.results(done))
     others = (("old_logps", old_logps), ("ref_logps", ref_logps))
-    q, count, (x, m, o, old, ref) = _sequences(logps, offsets, mask, others)
+    q, count, (x, m, o, old, ref) = _sequences(logps, offsets, mask, others, wide_grad)
     per_token = not (isinstance(advantages, torch.Tensor) and advantages.shape == (count, 1))
     _train.like("advantages", advantages, "logps (or [sequences, 1])", x.dtype, x.shape if per_token else (count, 1))
     dev = _train.on_gpu("logps", logps, (("offsets", offsets), ("mask", mask), ("advantages", advantages), *others))
-    L, adv = _train.load(), _dense(advantages)
-    f, kl, clipped = x.new_empty(3, dtype=_train.wide(x.dtype)).unbind()
-    grad = torch.empty_like(x)
+    L, adv, out = _train.load(), _dense(advantages), _train.wide(x.dtype)
+    f, kl, clipped = x.new_empty(3, dtype=out).unbind()
+    grad = torch.empty_like(x, dtype=out if wide_grad else x.dtype)
     size = L.lbfgs_train_sequences_workspace(q.tokens, count)
     ws = x.new_empty(size, dtype=torch.uint8) if size else None
     _train.enqueue(L.lbfgs_train_policy, dev, C.byref(q), x.data_ptr(), old.data_ptr(), _train.ptr(ref), adv.data_ptr(), per_token, clip_low, clip_high, kl_coef,
@@ -228,30 +234,31 @@ class _ValueAndGrad(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logps, result):
         ctx.save_for_backward(result.grad)
+        ctx.dtype = logps.dtype
         return result.f
 
     @staticmethod
     @once_differentiable
     def backward(ctx, up):
         _train.refuse_capture("the backward pass of a loss", "preference or policy")
-        (grad,) = ctx.saved_tensors
-        if grad.dtype == up.dtype:
-            return grad * up, None
-        return (grad.to(up.dtype) * up).to(grad.dtype), None  # (16 bits: what comes in is not rounded, the product is)
+        (grad,) = ctx.saved_tensors  # (in 32 bits or more, as what comes in: the product is rounded, once)
+        return (grad * up).to(ctx.dtype), None
 
 
-def _differentiable(name, logps, result):
-    if logps.requires_grad and torch.is_grad_enabled():
-        _train.refuse_capture(name + "_loss", name)
-        return _ValueAndGrad.apply(logps, result)
-    return result.f
+def _differentiable(name, function, logps, *others, **options):
+    wanted = isinstance(logps, torch.Tensor) and logps.requires_grad and torch.is_grad_enabled()
+    result = function(logps, *others, wide_grad=wanted, **options)
+    if not wanted:
+        return result.f
+    _train.refuse_capture(name + "_loss", name)
+    return _ValueAndGrad.apply(logps, result)
 
 
 def preference_loss(logps, ref_logps=None, **options):
     """`preference(...).f`, differentiable in logps (the reference is a constant)."""
-    return _differentiable("preference", logps, preference(logps, ref_logps, **options))
+    return _differentiable("preference", preference, logps, ref_logps, **options)
 
 
 def policy_loss(logps, old_logps, advantages, **options):
     """`policy(...).f`, differentiable in logps (old and reference log-probabilities and advantages are constants)."""
-    return _differentiable("policy", logps, policy(logps, old_logps, advantages, **options))
+    return _differentiable("policy", policy, logps, old_logps, advantages, **options)

@@ -507,6 +507,46 @@ def test_losses_autograd():
     assert not losses.policy_loss(lp, old, torch.ones(4, 1).cuda(), offsets=off, mask=mask).requires_grad
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("lengths", ["short", "chunk", "many", "ones", "wide", [70001, 60000, 3, 0, 90000, 8]])
+def test_16_bit_gradients_are_rounded_once(lengths, dtype):
+    """Slopes of 1/tokens and 1/(pairs length) are not rounded to 16 bits, where f16 has few steps for them or none, before what
+    comes into the loss -- a loss scale -- multiplies them.  In 32 bits as a direct result, too."""
+    t, up = DT[dtype], 65536.0
+    u, e, small = unit(t)
+    lp, old, off, mask, spans, keep = ragged(LENGTHS.get(lengths) if isinstance(lengths, str) else lengths, t, 30, masked=0.1)
+    scale = torch.tensor(up, device="cuda")
+    for strided in (False, True):  # (native, and the way through Python)
+        x = torch.stack((lp, lp), 1)[:, 0] if strided else lp.clone()
+        x.requires_grad_()
+        beta = 0.1
+        _, _, want, size = preference_in_64_bits(lp, old, spans, keep, beta, "logistic", 0.0, True)
+        sums = beta * beta * 4e-15 * (1 + float(size))
+        wide = losses.preference(x.detach(), old, offsets=off, mask=mask, beta=beta, normalize_lengths=True, wide_grad=True)
+        assert wide.grad.dtype == torch.float32
+        near(wide.grad, want, u * 1.01 * want.abs() + sums, "preference")
+        losses.preference_loss(x, old, offsets=off, mask=mask, beta=beta, normalize_lengths=True).backward(scale)
+        # a 32-bit slope, its product (a power of two) and one rounding to 16 bits
+        near(x.grad, want * up, (e + u) * 1.01 * (want * up).abs() + sums * up + small, "preference_loss")
+        for adv, reduction in ((torch.randn(lp.shape, generator=torch.Generator().manual_seed(1)).to(t).cuda(), "tokens"),
+                               (torch.randn(len(spans), 1, generator=torch.Generator().manual_seed(2)).to(t).cuda(), "sequences")):
+            _, _, _, want, parts, *_ = policy_in_64_bits(lp, old, adv, None, spans, keep, 0.2, 0.2, 0.0, reduction)
+            wide = losses.policy(x.detach(), old, adv, offsets=off, mask=mask, reduction=reduction, wide_grad=True)
+            assert wide.grad.dtype == torch.float32
+            near(wide.grad, want, u * 1.01 * want.abs() + 8 * u * parts, "policy")
+            x.grad = None
+            losses.policy_loss(x, old, adv, offsets=off, mask=mask, reduction=reduction).backward(scale)
+            near(x.grad, want * up, (e + u) * 1.01 * (want * up).abs() + 8 * u * parts * up + small, "policy_loss")
+
+
+def test_a_wide_gradient_of_wide_data_is_the_same():
+    lp, old, off, mask, _, _ = ragged(LENGTHS["short"], torch.float32, 3, masked=0.2)
+    for t in (torch.float32, torch.float64):
+        a, b = (losses.preference(lp.to(t), old.to(t), offsets=off, mask=mask, wide_grad=w) for w in (False, True))
+        c, d = (losses.policy(lp.to(t), old.to(t), old.to(t), offsets=off, mask=mask, wide_grad=w) for w in (False, True))
+        assert a.grad.dtype == b.grad.dtype == d.grad.dtype == t and torch.equal(a.grad, b.grad) and torch.equal(c.grad, d.grad)
+
+
 def test_losses_gradient_against_differences():
     lp, old, off, mask, spans, keep = ragged([9, 4, 6, 5], torch.float64, 5, masked=0.2)
     adv = torch.randn(24, dtype=torch.float64, generator=torch.Generator().manual_seed(0)).cuda()

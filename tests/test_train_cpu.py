@@ -176,6 +176,24 @@ def test_c_orthogonalize_refusals(lib):
     assert call(batch=0, g=None, out=None, ws=None) == 0 and call(m=0, g=None, out=None, ws=None) == 0
 
 
+def test_the_flag_of_a_wide_gradient(lib):
+    assert int(re.search(r"LBFGS_TRAIN_WIDE_GRAD = (\d+)", header()).group(1)) == _train.WIDE_GRAD
+    for dtype in (4, -1, 255, 512):
+        s = seqs(dtype=dtype | _train.WIDE_GRAD)
+        refused(lib.lbfgs_train_preference(s, P, P, 0.1, 0.0, 0, 0, P, P, P, P, 1 << 30, None), "element type")
+        refused(lib.lbfgs_train_policy(s, P, P, P, P, 1, 0.2, 0.2, 0.0, 0, P, P, P, P, P, 1 << 30, None), "element type")
+    for dtype in (0, 1, 2, 3):  # offered: what is wrong then is something else
+        s = seqs(dtype=dtype | _train.WIDE_GRAD)
+        refused(lib.lbfgs_train_preference(s, None, P, 0.1, 0.0, 0, 0, P, P, P, P, 1 << 30, None), "are needed")
+        refused(lib.lbfgs_train_policy(s, None, P, P, P, 1, 0.2, 0.2, 0.0, 0, P, P, P, P, P, 1 << 30, None), "are needed")
+    c = _train.calls()
+    for f, n in ((c.preference_wide, 8), (c.policy_wide, 10)):
+        with pytest.raises(TypeError, match=f"{n} are taken"):
+            f(*[0] * (n - 1))
+    x = torch.zeros(2, 8)
+    assert c.preference_wide(x, x, None, None, 0.1, 0.0, 0, False) is None and c.policy_wide(x, x, x, None, None, None, 0.2, 0.2, 0.0, 0) is None
+
+
 # ------------------------------------------------------------------------------------ Python functions
 def test_logprobs_refusals(lib):
     x, y = torch.zeros(2, 5), torch.zeros(2, dtype=torch.int64)
