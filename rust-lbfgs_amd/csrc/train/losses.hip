@@ -503,7 +503,7 @@ struct Policy {
     int per_token, by_sequence;
 };
 
-// e^q - 1 and e^q - 1 - q without their cancellation
+// e^q - 1 and e^q - 1 - q, where they would cancel by their series
 __device__ __forceinline__ void kl_terms(float q, float& em1, float& k) {
     if (fabsf(q) < 0.5f) {  // q^2 (1/2 + q/6 + ...): the first term left out is below 2^-24 of the sum
         k = q * q * (0.5f + q * (1.f / 6 + q * (1.f / 24 + q * (1.f / 120 + q * (1.f / 720 + q * (1.f / 5040 + q * (1.f / 40320)))))));
@@ -514,8 +514,26 @@ __device__ __forceinline__ void kl_terms(float q, float& em1, float& k) {
     }
 }
 __device__ __forceinline__ void kl_terms(double q, double& em1, double& k) {
-    em1 = expm1(q);
-    k = em1 - q;
+    if (fabs(q) < 0.5) {  // ... to q^15/15!: 2^-57
+        double p = 1.0 / 1307674368000;
+        p = fma(p, q, 1.0 / 87178291200);
+        p = fma(p, q, 1.0 / 6227020800);
+        p = fma(p, q, 1.0 / 479001600);
+        p = fma(p, q, 1.0 / 39916800);
+        p = fma(p, q, 1.0 / 3628800);
+        p = fma(p, q, 1.0 / 362880);
+        p = fma(p, q, 1.0 / 40320);
+        p = fma(p, q, 1.0 / 5040);
+        p = fma(p, q, 1.0 / 720);
+        p = fma(p, q, 1.0 / 120);
+        p = fma(p, q, 1.0 / 24);
+        p = fma(p, q, 1.0 / 6);
+        k = q * q * fma(p, q, 0.5);
+        em1 = q + k;
+    } else {
+        em1 = expm1(q);
+        k = em1 - q;
+    }
 }
 
 // tokens of each sequence that count -> 1 / their number; kept tokens and sequences with any of this workgroup

@@ -444,6 +444,28 @@ def test_small_kl_terms_do_not_cancel():
     assert abs(float(r.kl) - float(want)) <= 11 * 2.0 ** -24 * float(want)
 
 
+@pytest.mark.parametrize("dtype", ["f64", "f32"])
+@pytest.mark.parametrize("q", [1e-12, 1e-9, 1e-6, 1e-3, 0.03, 0.2, 0.499, 0.501, 0.9, 2.0, 5.0])
+def test_kl_terms_of_every_size(q, dtype):
+    """e^q - 1 - q against its series in exact fractions: relative to itself, from where it is 10^-24 to where e^q is all of it."""
+    from fractions import Fraction
+
+    t = DT[dtype]
+    u, e, _ = unit(t)
+    for q_ in (float(torch.tensor(v, dtype=t)) for v in (q, -q, 0.7 * q, -0.7 * q)):
+        x, k, term, n = Fraction(q_), Fraction(0), Fraction(1), 1
+        while n <= 60:
+            term = term * x / n
+            k += term if n > 1 else 0
+            n += 1
+        z = torch.zeros(1, 7, dtype=t, device="cuda")
+        r = losses.policy(z, z, z, ref_logps=z + q_, kl_coef=1.0)
+        # the exponential's rounding and the difference's beside it (|e^q - 1| / k < 4.5 from 0.5 on), the series' below, the mean's
+        assert abs(float(r.kl) - float(k)) <= 12 * u * float(k), q_
+        want = -float(k + x) / 7  # dk/dlogp, of one token of seven
+        assert (r.grad.double() + (-want)).abs().max() <= (8 * u + e) * abs(want), q_
+
+
 @pytest.mark.parametrize("bits", [32, 64])
 def test_bad_offsets_give_nan(bits):
     """Offsets are data of the device: bad ones are clamped to the tokens there are, and the loss says so."""
