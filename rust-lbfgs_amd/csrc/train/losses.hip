@@ -503,39 +503,6 @@ struct Policy {
     int per_token, by_sequence;
 };
 
-// e^q - 1 and e^q - 1 - q, where they would cancel by their series
-__device__ __forceinline__ void kl_terms(float q, float& em1, float& k) {
-    if (fabsf(q) < 0.5f) {  // q^2 (1/2 + q/6 + ...): the first term left out is below 2^-24 of the sum
-        k = q * q * (0.5f + q * (1.f / 6 + q * (1.f / 24 + q * (1.f / 120 + q * (1.f / 720 + q * (1.f / 5040 + q * (1.f / 40320)))))));
-        em1 = q + k;
-    } else {
-        em1 = expf(q) - 1.f;
-        k = em1 - q;
-    }
-}
-__device__ __forceinline__ void kl_terms(double q, double& em1, double& k) {
-    if (fabs(q) < 0.5) {  // ... to q^15/15!: 2^-57
-        double p = 1.0 / 1307674368000;
-        p = fma(p, q, 1.0 / 87178291200);
-        p = fma(p, q, 1.0 / 6227020800);
-        p = fma(p, q, 1.0 / 479001600);
-        p = fma(p, q, 1.0 / 39916800);
-        p = fma(p, q, 1.0 / 3628800);
-        p = fma(p, q, 1.0 / 362880);
-        p = fma(p, q, 1.0 / 40320);
-        p = fma(p, q, 1.0 / 5040);
-        p = fma(p, q, 1.0 / 720);
-        p = fma(p, q, 1.0 / 120);
-        p = fma(p, q, 1.0 / 24);
-        p = fma(p, q, 1.0 / 6);
-        k = q * q * fma(p, q, 0.5);
-        em1 = q + k;
-    } else {
-        em1 = expm1(q);
-        k = em1 - q;
-    }
-}
-
 // tokens of each sequence that count -> 1 / their number; kept tokens and sequences with any of this workgroup
 template <class Q>
 __device__ __forceinline__ void sequence_weights(const Q& q, const Space& sp, int block, int blocks) {
@@ -602,50 +569,54 @@ __device__ __forceinline__ void all_counts(const Space& sp, int blocks, double& 
     if (some < 1) some = 1;
 }
 
-// e^d in 64 bits, to 2^-42: d = n log 2 + r, a polynomial of r, the power of two.  (The library's is right to the last of 53 bits,
-// which for ratios of 32-bit values nobody sees, and takes twice as long.)  Beyond the range, infinities and NaN: the library's.
-__device__ __forceinline__ double exp_of(double d) {
-    if (!(fabs(d) < 600)) return exp(d);
-    const double n = rint(d * 1.4426950408889634);
-    const double r = fma(n, -2.3190468138462996e-17, fma(n, -0.6931471805599453, d));  // log 2 and what a double leaves of it
-    double p = 1.0 / 3628800;  // the Taylor series to r^10, |r| < 0.347: the first term left out is below 2^-42 of r / 11
-    p = fma(p, r, 1.0 / 362880);
-    p = fma(p, r, 1.0 / 40320);
-    p = fma(p, r, 1.0 / 5040);
-    p = fma(p, r, 1.0 / 720);
-    p = fma(p, r, 1.0 / 120);
-    p = fma(p, r, 1.0 / 24);
-    p = fma(p, r, 1.0 / 6);
-    p = fma(p, r, 0.5);
-    p = fma(p, r, 1.0);
-    p = fma(p, r, 1.0);
-    return ldexp(p, (int)n);
-}
-// Of a token's log-probabilities: r A, and whether the border that its advantage goes with is passed.  In 32 bits where that is as good
-// -- the difference itself, and r - 1 for a small one, so that r is right to 2^-22 |r - 1| -- and in 64 where it is not: at the border
-// (the gradient jumps there), and for a large difference.
-__device__ __forceinline__ void ratio(const Policy& o, float lp, float old, double a, bool& over, double& ra) {
-    const float d = lp - old;
-    const double border = a > 0 ? o.log_high : o.log_low;
-    const float b = (float)border;
-    over = a > 0 ? d > b : a < 0 && d < b;
-    if (!(fabsf(d - b) > 1e-6f * fabsf(b))) {  // (d and b are within 2^-23 of what they stand for)
-        const double e = (double)lp - (double)old;
-        over = a > 0 ? e > border : a < 0 && e < border;
+// e^x, e^x - 1 and e^x - 1 - x, each of itself: to 2^-50 for 64-bit data, and to 2^-32 for others, whose results have 24 bits.
+//   x = n log 2 + r, with n = 0 and r = x below 1/2;   t = e^r - 1 - r = r^2 (1/2 + r/6 + ...);   e^x = 2^n (1 + r + t);
+// of n = 0 the others are r + t and t, where they would cancel.  No branch: in most waves one of 64 differences is beyond 1/2.  Of 32-bit
+// data the series is 32-bit from r^5/120 on, to r^11: 2^-24 of that is 2^-32 of t.  (With the terms in 32 bits throughout the pass over 8.4
+// million tokens took 2 us less, 49.5, and the KL term and its slope were off by six roundings of the result.)
+template <class T>
+struct Exponential {
+    double x, e, rt, t;
+    bool near;
+    __device__ __forceinline__ explicit Exponential(double x_) : x(x_) {
+        const double xc = __builtin_fmin(__builtin_fmax(x, -1000.0), 1000.0);  // (e^x is 0 or infinite there; and of a NaN some number)
+        near = fabs(xc) < 0.5;
+        const double n = near ? 0 : rint(xc * 1.4426950408889634);
+        const double r = fma(n, -2.3190468138462996e-17, fma(n, -0.6931471805599453, xc));  // log 2 and what a double leaves of it
+        double p;
+        if constexpr (sizeof(T) == 8) {
+            p = 1. / 1307674368000.;  // 15!
+            p = fma(p, r, 1. / 87178291200.);
+            p = fma(p, r, 1. / 6227020800.);
+            p = fma(p, r, 1. / 479001600.);
+            p = fma(p, r, 1. / 39916800.);
+            p = fma(p, r, 1. / 3628800.);
+            p = fma(p, r, 1. / 362880.);
+            p = fma(p, r, 1. / 40320.);
+            p = fma(p, r, 1. / 5040.);
+            p = fma(p, r, 1. / 720.);
+            p = fma(p, r, 1. / 120.);
+            p = fma(p, r, 1. / 24.);
+        } else {
+            const float h = (float)r;
+            float c = 1.f / 39916800.f;  // 11!
+            c = fmaf(c, h, 1.f / 3628800.f);
+            c = fmaf(c, h, 1.f / 362880.f);
+            c = fmaf(c, h, 1.f / 40320.f);
+            c = fmaf(c, h, 1.f / 5040.f);
+            c = fmaf(c, h, 1.f / 720.f);
+            c = fmaf(c, h, 1.f / 120.f);
+            p = fma((double)c, r, 1. / 24.);
+        }
+        p = fma(p, r, 1. / 6.);
+        t = r * r * fma(p, r, 0.5);
+        rt = r + t;
+        e = ldexp(1 + rt, (int)n);
+        if (x != x) e = t = x;
     }
-    if (fabsf(d) < 0.5f) {
-        float em1, k;
-        kl_terms(d, em1, k);
-        ra = fma((double)em1, a, a);
-    } else {
-        ra = a == 0 && d == d ? 0 : exp_of((double)lp - (double)old) * a;  // (an advantage of 0 gives 0 for any ratio, one that overflowed too)
-    }
-}
-__device__ __forceinline__ void ratio(const Policy& o, double lp, double old, double a, bool& over, double& ra) {
-    const double d = lp - old;
-    over = (a > 0 && d > o.log_high) || (a < 0 && d < o.log_low);
-    ra = a == 0 && d == d ? 0 : exp(d) * a;
-}
+    __device__ __forceinline__ double value() const { return e; }
+    __device__ __forceinline__ void less(double& em1, double& k) const { em1 = near ? rt : e - 1, k = near ? t : em1 - x; }
+};
 
 template <class T, class G>
 struct PolicyData {
@@ -667,23 +638,22 @@ struct PolicyTokens {
     }
 };
 
-// L = -min(r A, clip(r) A) + kl (e^q - 1 - q) with r = e^d, d = logp - old, q = ref - logp.  Products with A, sums and the slope are taken in 64
-// bits (the slope is rounded once, to the gradient's type): advantages have mean 0, and the mean of r A is what is left of terms a thousand
-// times larger.
+// L = -min(r A, clip(r) A) + kl (e^q - 1 - q) with r = e^d, d = logp - old, q = ref - logp.  All of it in 64 bits, the slope rounded once, to
+// the gradient's type: advantages have mean 0, and the mean of r A is what is left of terms a thousand times larger; where they are 0, as a
+// group of equal rewards has them, the KL term is all there is; and at the border that an advantage goes with the gradient jumps.
 template <class T>
 __device__ __forceinline__ void token(const Policy& o, T lp, T old, T ref, double a, double weight, double& slope, double& f, double& kl, double& clipped) {
-    typedef typename Num<T>::acc A;
-    bool over;
-    double ra;
-    ratio(o, (A)lp, (A)old, a, over, ra);
+    const double d = (double)lp - (double)old;
+    const bool over = a > 0 ? d > o.log_high : a < 0 && d < o.log_low;
+    const double ra = a == 0 && d == d ? 0 : Exponential<T>(d).value() * a;  // (an advantage of 0 gives 0 for any ratio, one that overflowed too)
     double loss = over ? -(a > 0 ? o.high : o.low) * a : -ra;
     slope = over ? 0 : -ra;
     if (o.kl != 0) {
-        A em1, term;
-        kl_terms((A)ref - (A)lp, em1, term);
-        loss += o.kl * (double)term;
-        slope -= o.kl * (double)em1;
-        kl += (double)term;
+        double em1, term;
+        Exponential<T>((double)ref - (double)lp).less(em1, term);
+        loss += o.kl * term;
+        slope -= o.kl * em1;
+        kl += term;
     }
     f += loss * weight;
     clipped += over;

@@ -466,6 +466,26 @@ def test_kl_terms_of_every_size(q, dtype):
         assert (r.grad.double() + (-want)).abs().max() <= (8 * u + e) * abs(want), q_
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("lengths", ["short", "many", "wide"])
+def test_policy_terms_have_64_bits(lengths, dtype):
+    """A gradient of 32 bits is off by its own rounding, of 2^-24, and 2^-32 of what it is made of: the ratio and the KL term alone too,
+    as where a group's advantages are 0."""
+    t, u = DT[dtype], 2.0 ** -24
+    lp, old, off, mask, spans, keep = ragged(LENGTHS[lengths], t, 40, masked=0.2)
+    gen = torch.Generator().manual_seed(4)
+    ref = (torch.nan_to_num(lp.float().cpu(), nan=0.0) + 0.3 * torch.randn(lp.shape, generator=gen)).to(t).cuda()
+    adv = torch.randn(len(spans), 1, generator=gen).to(t).cuda()
+    tokens = torch.randn(lp.shape, generator=gen).to(t).cuda()
+    for a, kl_coef, reduction in ((0 * adv, 0.1, "tokens"), (0 * tokens, 0.1, "tokens"), (0 * adv, 1.0, "sequences"), (adv, 0.0, "tokens"), (tokens, 0.0, "tokens"), (tokens, 0.3, "sequences")):
+        r = losses.policy(lp, old, a, ref_logps=ref, offsets=off, mask=mask, kl_coef=kl_coef, reduction=reduction, wide_grad=True)
+        f, kl, clip, grad, parts, size, klsize, _ = policy_in_64_bits(lp, old, a, ref, spans, keep, 0.2, 0.2, kl_coef, reduction)
+        what = (lengths, dtype, kl_coef, reduction)
+        near(r.grad, grad, 1.01 * u * grad.abs() + 2.0 ** -32 * parts, what)
+        near(r.f, f, 1.01 * u * f.abs() + 2.0 ** -32 * (size + klsize), what)
+        near(r.kl, kl, 1.01 * u * kl.abs(), what)
+
+
 @pytest.mark.parametrize("bits", [32, 64])
 def test_bad_offsets_give_nan(bits):
     """Offsets are data of the device: bad ones are clamped to the tokens there are, and the loss says so."""
