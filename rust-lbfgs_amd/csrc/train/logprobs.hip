@@ -179,11 +179,23 @@ __device__ __forceinline__ void put(T* dx, const Pack<T, N>& d) {
     else
         *to = *(const uint4_*)&d;
 }
+// exp((x - hi)/tau) with c + c_lo = log2(e)/tau.  Of 32-bit logits what the difference and its product round away is made up for:
+// of 50 powers of e down, that was 40 roundings of the gradient.  (16-bit gradients round by more than it, and the pass waits for memory.)
+template <class T, class A>
+__device__ __forceinline__ A power(A x, A hi, A c, A c_lo) {
+    const A e = x - hi, p = e * c, v = exp2_of(p);
+    if constexpr (sizeof(T) == 4) {
+        const A b = e - x, e_lo = (x - (e - b)) - (hi + b);
+        const A p_lo = fmaf(e_lo, c, fmaf(e, c_lo, fmaf(e, c, -p)));
+        return p > -200 ? fmaf(v, p_lo * 0.69314718f, v) : v;  // (0 beyond, and at -inf, where p_lo is NaN)
+    }
+    return v;
+}
 template <bool PAST, class T, int N, class A>
-__device__ __forceinline__ void grad_pack(const Pack<T, N>& p, T* dx, int64_t v, int64_t y, A hi, A c, A scale, A at_target) {
+__device__ __forceinline__ void grad_pack(const Pack<T, N>& p, T* dx, int64_t v, int64_t y, A hi, A c, A c_lo, A scale, A at_target) {
     Pack<T, N> d;
 #pragma unroll
-    for (int k = 0; k < N; k++) d.v[k] = (T)(scale * exp2_of(((A)p.v[k] - hi) * c));
+    for (int k = 0; k < N; k++) d.v[k] = (T)(scale * power<T, A>((A)p.v[k], hi, c, c_lo));
     const uint64_t off = (uint64_t)(y - v);
     if (off < (uint64_t)N) {
 #pragma unroll
@@ -197,7 +209,7 @@ __device__ __forceinline__ void grad_pack(const Pack<T, N>& p, T* dx, int64_t v,
 }
 
 template <class T, int BLOCK, bool PAST>
-__global__ __launch_bounds__(BLOCK) void logprobs_grad_kernel(const T* x, Rows r, double tau, typename Num<T>::acc c, int splits, int64_t part,
+__global__ __launch_bounds__(BLOCK) void logprobs_grad_kernel(const T* x, Rows r, double tau, typename Num<T>::acc c, typename Num<T>::acc c_lo, int splits, int64_t part,
                                                               const double* lse, const typename Num<T>::acc* grad, T* dx) {
     typedef typename Num<T>::acc A;
     constexpr int N = vec_len<T>(), U = 4;
@@ -236,11 +248,11 @@ __global__ __launch_bounds__(BLOCK) void logprobs_grad_kernel(const T* x, Rows r
 #pragma unroll
             for (int u = 0; u < U; u++) p[u] = *(const Pack<T, N>*)(in + head + (i + u * BLOCK) * N);
 #pragma unroll
-            for (int u = 0; u < U; u++) grad_pack<PAST, T, N, A>(p[u], out, head + (i + u * BLOCK) * N, y, hi, c, scale, at_target);
+            for (int u = 0; u < U; u++) grad_pack<PAST, T, N, A>(p[u], out, head + (i + u * BLOCK) * N, y, hi, c, c_lo, scale, at_target);
         }
-        for (; i < packs; i += BLOCK) grad_pack<PAST, T, N, A>(*(const Pack<T, N>*)(in + head + i * N), out, head + i * N, y, hi, c, scale, at_target);
-        for (int64_t k = lo + tid; k < head; k += BLOCK) grad_pack<PAST, T, 1, A>({{in[k]}}, out, k, y, hi, c, scale, at_target);
-        for (int64_t k = done + tid; k < hi_v; k += BLOCK) grad_pack<PAST, T, 1, A>({{in[k]}}, out, k, y, hi, c, scale, at_target);
+        for (; i < packs; i += BLOCK) grad_pack<PAST, T, N, A>(*(const Pack<T, N>*)(in + head + i * N), out, head + i * N, y, hi, c, c_lo, scale, at_target);
+        for (int64_t k = lo + tid; k < head; k += BLOCK) grad_pack<PAST, T, 1, A>({{in[k]}}, out, k, y, hi, c, c_lo, scale, at_target);
+        for (int64_t k = done + tid; k < hi_v; k += BLOCK) grad_pack<PAST, T, 1, A>({{in[k]}}, out, k, y, hi, c, c_lo, scale, at_target);
     }
 }
 
@@ -297,7 +309,7 @@ static void launch_forward(const void* x, const Rows& r, double tau, void* logps
 template <class T>
 static void launch_grad(const void* x, const Rows& r, double tau, const double* lse, const void* grad, void* dx, hipStream_t s) {
     typedef typename Num<T>::acc A;
-    const A c = (A)(1.4426950408889634 / tau);
+    const A c = (A)(1.4426950408889634 / tau), c_lo = (A)(1.4426950408889634 / tau - (double)c);
     const int64_t bytes = r.vocab * (int64_t)sizeof(T);
     // Workgroups to a row: so many that there are 512 of 16 KiB at least, or 2048 of 64 KiB.  Measured for one to a row, 512 and 2048 in all,
     // in us: in bf16 64 rows of 131072 16.6, 6.7, 9.8, 1 row 14.5, 3.2, 3.3, 255 rows of 32768 9.3, 6.9, 9.8, 1000 of 8192 6.9, 6.9, 9.8; in
@@ -308,7 +320,7 @@ static void launch_grad(const void* x, const Rows& r, double tau, const double* 
     splits = (r.vocab + part - 1) / part;
     const int64_t units = r.rows * splits;
     const unsigned grid = (unsigned)(units < MOST_BLOCKS ? units : MOST_BLOCKS);
-    auto launch = [&](auto kernel, int block) { kernel<<<grid, block, 0, s>>>((const T*)x, r, tau, c, (int)splits, part, lse, (const A*)grad, (T*)dx); };
+    auto launch = [&](auto kernel, int block) { kernel<<<grid, block, 0, s>>>((const T*)x, r, tau, c, c_lo, (int)splits, part, lse, (const A*)grad, (T*)dx); };
     if (bytes <= 4096)  // (many short rows: no logits worth keeping)
         launch(logprobs_grad_kernel<T, 64, false>, 64);
     else if ((double)r.rows * bytes < PAST_CACHES)

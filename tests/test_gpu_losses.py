@@ -137,6 +137,27 @@ def test_logprobs_extreme_temperatures(dtype, taus):
         assert ((d - (onehot - p)).abs() <= 1e-6 + torch.finfo(x.dtype).eps / 2).all(), tau
 
 
+@pytest.mark.parametrize("tau", [1.0, 0.7, 3.0])
+def test_small_probabilities_have_gradients_of_full_precision(tau):
+    """Of 32-bit logits, relative to each gradient: the upstream one over tau, exp(-l) and their product 3 roundings, the hardware's
+    exponential 2 (an ulp), what makes up for its argument's rounding 1, the product 1.  Down to 60 powers of e, beside logits of any size."""
+    u = 2.0 ** -24
+    for V, shift in ((4099, 0.0), (700, 1000.3), (50001, -7.1)):
+        gen = torch.Generator().manual_seed(V)
+        x = (shift - 60 * tau * torch.rand(9, V, generator=gen)).cuda()
+        x[0, 5:9], x[1, 3] = -math.inf, torch.finfo(torch.float32).min
+        y, g = torch.randint(20, V, (9,), generator=gen).cuda(), torch.randn(9, generator=gen).cuda()
+        z = x.double()
+        m = z.amax(-1, keepdim=True)
+        w = ((z - m) / tau).exp()
+        lse = torch.cat((m, w.sum(-1, keepdim=True).log()), 1)
+        dx = losses.token_logprobs_grad(x, y, lse, g, tau)
+        want = -(g.double() / tau).unsqueeze(-1) * w / w.sum(-1, keepdim=True)
+        off = ((dx.double() - want).abs() - 8 * u * want.abs()).scatter(-1, y.unsqueeze(-1), 0.0)
+        assert off.max() <= 0, (V, float(((dx.double() - want) / want).abs().scatter(-1, y.unsqueeze(-1), 0.0).nan_to_num(0.0).max() / u))
+        assert (dx[0, 5:9] == 0).all() and dx[1, 3] == 0
+
+
 def test_what_comes_into_a_loss_is_not_rounded_to_16_bits():
     for dtype in (torch.bfloat16, torch.float16):
         x = torch.randn(4, 700, generator=torch.Generator().manual_seed(0)).cuda().to(dtype).requires_grad_()
