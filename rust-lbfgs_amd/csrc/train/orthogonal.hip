@@ -163,7 +163,7 @@ __device__ __forceinline__ int place(int row, int chunk) {
 // One such copy: 16 bytes a lane from base + off to 1024 bytes of LDS.  Written out, because the compiler takes
 // any LDS read behind its own form of it as one that has to wait for all copies; the waits are the kernel's (ready()).
 __device__ __forceinline__ void copy_to_lds(const f16* base, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "m0");
 }
 __device__ __forceinline__ const f16* uniform(const f16* p) {  // (the same in all lanes: to scalar registers)
     const uint64_t a = (uint64_t)p;

@@ -60,6 +60,20 @@ def test_no_kernel_uses_scratch_memory(lib):
     assert len(sizes) >= 40 and set(sizes) == {"0"}
 
 
+def test_inline_assembly_names_the_special_registers_it_writes():
+    """What the compiler is not told of it may keep something in."""
+    found = 0
+    for unit in _build.TRAIN_SRCS:
+        for text in re.findall(r"\basm\b\s*(?:volatile)?\s*\((.*?)\);", open(unit).read(), flags=re.S):
+            clobbers = text.rsplit(":", 1)[1] if text.count(":") >= 3 else ""
+            for instruction in re.split(r"\\n|;", text.split(":")[0].replace("\\t", " ").replace('"', " ")):
+                for register in ("m0", "vcc", "exec", "scc"):
+                    if re.match(r"\s*\w+ " + register + r"\b", instruction):
+                        found += 1
+                        assert f'"{register}"' in clobbers, (unit, text)
+    assert found  # the copies to LDS
+
+
 def test_the_library_is_rebuilt_when_its_sources_differ(lib, monkeypatch):
     monkeypatch.setattr(_build, "train_build_id", lambda: "0" * 16)
     monkeypatch.setattr(_train, "_LIB", None)
