@@ -1,6 +1,9 @@
 """Directions for matrix parameters, beside the optimiser's own for vectors (the two-loop recursion, the orthant projection).
 
-    d = directions.orthogonalize(-gradient.view(rows, cols))      # every singular value brought near 1
+    d = directions.orthogonalize(-gradient.view(rows, cols).float())      # every singular value brought near 1
+
+The optimiser's gradients are float64, an orthogonalised update is not: it is a step of a descent of its own over matrices, and the polynomial
+leaves singular values tens of percent apart.
 
 Kernels: rust-lbfgs_amd/csrc/train/orthogonal.hip behind include/lbfgs_train.h.
 """

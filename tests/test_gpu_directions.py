@@ -367,3 +367,14 @@ def test_an_orthogonalised_descent_step():
         with torch.no_grad():
             W.sub_(0.02 * d)
     assert W.isfinite().all()
+
+
+def test_the_example_takes_the_optimisers_gradients():
+    import re
+
+    example = re.search(r"    d = (directions\.orthogonalize\(.*\))  ", directions.__doc__).group(1)
+    g = torch.randn(30 * 50, dtype=torch.float64, generator=torch.Generator().manual_seed(0)).cuda()
+    d = eval(example, dict(directions=directions, gradient=g, rows=30, cols=50))
+    used = -g.view(30, 50).float()
+    want, trail = in_64_bits(used, 5, ABC)
+    assert d.dtype == torch.float32 and float((d.double().cpu() - want.cpu()).norm()) <= tolerance(used, trail, ABC, d.dtype) * float(want.norm())

@@ -281,6 +281,14 @@ def test_orthogonalize_refusals(lib):
         directions.orthogonalize(torch.zeros(2, 3), coefficients=(1.0, 2.0))
 
 
+def test_the_example_of_a_direction_takes_the_optimisers_gradients(lib):
+    """float64, as every gradient that the optimiser has; with one of the CPU what is wrong is the device alone."""
+    example = re.search(r"    d = (directions\.orthogonalize\(.*\))  ", directions.__doc__).group(1)
+    names = dict(directions=directions, gradient=torch.ones(6, dtype=torch.float64), rows=2, cols=3)
+    with pytest.raises(TypeError, match="no CPU fallback"):
+        eval(example, names)
+
+
 def test_views_with_a_sign_to_come_are_refused(lib):
     lazy = torch.view_as_complex(torch.ones(6, 2)).conj().imag
     assert lazy.is_neg()
