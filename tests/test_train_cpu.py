@@ -289,6 +289,15 @@ def test_the_example_of_a_direction_takes_the_optimisers_gradients(lib):
         eval(example, names)
 
 
+def test_what_is_said_of_the_default_coefficients():
+    smallest, low, high = re.search(r"below 1/(\d+) of the norm\) into ([0-9.]+) \.\. ([0-9.]+)\.\n", directions.orthogonalize.__doc__).groups()
+    s = torch.linspace(1 / int(smallest), 1, 1000001, dtype=torch.float64)
+    a, b, c = directions.COEFFICIENTS
+    for _ in range(5):
+        s = a * s + b * s ** 3 + c * s ** 5
+    assert float(low) <= float(s.min()) < float(low) + 0.01 and float(high) - 0.01 < float(s.max()) <= float(high)
+
+
 def test_views_with_a_sign_to_come_are_refused(lib):
     lazy = torch.view_as_complex(torch.ones(6, 2)).conj().imag
     assert lazy.is_neg()
