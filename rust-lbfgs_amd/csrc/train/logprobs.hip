@@ -5,7 +5,8 @@
 // Both are bound by HBM: the forward pass reads every logit once (running maximum and sum in registers), the gradient
 // reads it once more and writes as much.  Measured in bf16 (a copy of 2 GiB: 4.93 TB/s, read and written): 8192 x 131072 forward
 // 347 us, 6.2 TB/s; 8192 x 32768 forward 79 to 110 us, 4.8 TB/s and more, gradient 173 us, 6.2 TB/s, part of what both read being in the
-// caches yet; 1020 rows of 50001 in 32 bits, 16-byte loads at any alignment, 28 and 56 us.  Few rows are bound by the launch: 8 of 32768 5.
+// caches yet; 1020 rows of 50001 in 32 bits, 16-byte loads at any alignment, 29 and 57 us; 4096 x 32768 in 64 bits
+// 210 and 380, 5.1 and 5.6 TB/s.  Few rows are bound by the launch: 8 of 32768 5.
 #include "common.h"
 
 #include <algorithm>
@@ -258,7 +259,7 @@ __global__ __launch_bounds__(BLOCK) void logprobs_grad_kernel(const T* x, Rows r
 
 // ------------------------------------------------------------------------------------ launches
 // A gradient of so many bytes is stored past the caches (half of the last one's 256 MB: a smaller one may be there for whoever reads it
-// next).  Forward and gradient of other logits in every pass: 8192 x 32768 in bf16 254 us (294 through the caches), 1020 x 50001 in f32 104 (119).
+// next).  Forward and gradient of other logits in every pass: 8192 x 32768 in bf16 254 us (294 through the caches), 1020 x 50001 in f32 102 (118).
 constexpr double PAST_CACHES = 128e6;
 constexpr int64_t MOST_BLOCKS = 1 << 22;  // a launch has less than 2^32 threads: kernels loop beyond
 
@@ -313,7 +314,7 @@ static void launch_grad(const void* x, const Rows& r, double tau, const double* 
     const int64_t bytes = r.vocab * (int64_t)sizeof(T);
     // Workgroups to a row: so many that there are 512 of 16 KiB at least, or 2048 of 64 KiB.  Measured for one to a row, 512 and 2048 in all,
     // in us: in bf16 64 rows of 131072 16.6, 6.7, 9.8, 1 row 14.5, 3.2, 3.3, 255 rows of 32768 9.3, 6.9, 9.8, 1000 of 8192 6.9, 6.9, 9.8; in
-    // f32, forward and gradient, 1020 of 50001 123, 123, 117 (all of them through the caches).
+    // f32, forward and gradient, 1020 of 50001 124, 124, 118 (all of them through the caches).
     auto shares = [&](int64_t all, int64_t least) { return std::min(all / r.rows, bytes / least); };
     int64_t splits = std::max<int64_t>({1, shares(512, 16384), shares(2048, 65536)});
     const int64_t part = part_of(r.vocab, (int)splits);

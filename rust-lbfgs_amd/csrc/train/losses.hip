@@ -2,7 +2,8 @@
 // with their gradients.
 //
 // The sequences are ragged, so tokens -- not sequences -- are dealt to the workgroups: a CHUNK of adjacent tokens each,
-// whatever sequences they belong to.  One answer of 100 000 tokens then occupies the chip as well as 10 000 of ten.
+// whatever sequences they belong to.  One answer of 100 000 tokens then occupies the chip as well as 10 000 of ten.  (Its chunks' records are
+// added up by one lane or by eight, by the mean length: one of 2 million among 1000 of 20 takes 85 us where 1000 of 2000 take 20.)
 // What a chunk finds about its sequences (sums, counts) it leaves as
 //     total[s]  for a sequence that lies inside the chunk,
 //     tail[w]   for the one that starts in chunk w and goes on,       head[w]  for the one that started before chunk w,
@@ -10,7 +11,8 @@
 // Every sum over tokens is held in 64 bits: the values wanted are differences of sums of thousands of terms.
 //
 // Large batches are bound by HBM, all others by launches and by how few loads wait for each other.  Measured in 32 bits: policy,
-// 8.4 million tokens, a reference and a mask: 7 us to count, 32 for losses and gradients (5.5 TB/s), 5 for the results; preference,
+// 8.4 million tokens, a reference and a mask: 7 us to count, 36 for losses and gradients (4.9 TB/s), 5 for the results -- by sequences 17, 52
+// (two exponentials of 64 bits a token, and the search) and 10 --; preference,
 // 48 sequences of up to 131072 tokens: sums 8 us (3.7 TB/s), slopes, loss and gradient 15; 512 of up to 2047: 5 and 6 us.
 #include "common.h"
 
@@ -715,7 +717,7 @@ __global__ __launch_bounds__(BLOCK) void policy_kernel(Seqs q, Policy o, PolicyD
 }
 // The mean over all tokens with an advantage for each: nothing is a sequence's own, all tokens from the first offset to the last are
 // alike, and nobody looks for their sequences.  One pack of 16 bytes of each tensor a thread.  2048 x 4096 tokens in 32 bits with a
-// reference: 30.1 us in all (36.3 by the pass that knows sequences).
+// reference: 45 us in all (53 by the pass that knows sequences), with a mask 51 (59).
 constexpr int ALIKE_BLOCKS = 1280;  // five to a compute unit
 template <class T, class G>
 __global__ __launch_bounds__(BLOCK) void policy_alike_kernel(Seqs q, Policy o, PolicyData<T, G> x, int count_blocks, Space sp) {
@@ -809,8 +811,8 @@ __global__ __launch_bounds__(BLOCK) void policy_small_kernel(Seqs whole, Policy 
 
 // ------------------------------------------------------------------------------------ launches
 // Up to so many tokens and sequences one workgroup does the whole of a loss, without a workspace.  Measured, whole calls one after the
-// other, in us (as several launches in brackets): 8 sequences of 60 tokens, preference 7.4 (10.3), policy 7.5 (13.7); 2 of 2048, 9.2 (10.3)
-// and 9.7 (13.8), with a mask and a mean of means 13.0 (16.5); 256 of 16, 11.0 (10.3), 12.2 (13.8) and 17.9 (16.8).
+// other, in us (as several launches in brackets): 8 sequences of 60 tokens, preference 7.6 (10.9), policy 8.1 (13.9); 2 of 2048, 9.4 (10.3)
+// and 10.4 (13.8), with a mask and a mean of means 13.1 (18.0); 256 of 16, 11.3 (11.2), 11.6 (14.3) and 18.1 (19.7).
 static bool small(int64_t tokens, int64_t seqs) { return tokens <= SMALL_TOKENS && seqs <= SMALL_SEQS; }
 
 static int64_t chunks_of(int64_t tokens) { return (tokens + CHUNK - 1) / CHUNK; }

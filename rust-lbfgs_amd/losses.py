@@ -193,7 +193,7 @@ def preference(logps, ref_logps=None, *, offsets=None, mask=None, beta=0.1, kind
 
 class Policy(NamedTuple):
     f: torch.Tensor              # the loss
-    kl: torch.Tensor             # mean of exp(q) - 1 - q, q = ref_logps - logps, over the tokens that count
+    kl: torch.Tensor             # mean of exp(q) - 1 - q, q = ref_logps - logps, over the tokens that count; 0 without a KL term in f
     clip_fraction: torch.Tensor  # share of them whose ratio is clipped
     grad: torch.Tensor           # df/dlogps
 

@@ -362,6 +362,15 @@ def test_preference_of_many_long_sequences(count, monkeypatch):
     test_preference("many long", "packed", "f32")
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("lengths", [[20] * 999 + [300001], [300001] + [3] * 1400 + [0], [7] * 100 + [40000, 0] + [1] * 98])
+def test_one_very_long_sequence_among_many_short(lengths, dtype, monkeypatch):
+    """The mean length is short, so one lane adds up the records of the long one's chunks."""
+    monkeypatch.setitem(LENGTHS, "one long", lengths)
+    test_preference("one long", "packed", dtype)
+    test_policy("one long", "packed", dtype)
+
+
 def test_preference_extreme_margins():
     """Margins far beyond where exp overflows, and an infinite one."""
     lp = torch.tensor([[0.0], [-2e4], [-1e30], [-math.inf], [-2e4], [0.0], [0.0], [0.0]], dtype=torch.float64).cuda()
